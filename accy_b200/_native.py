@@ -70,6 +70,9 @@ PROTOTYPES = {
     "accy_b200_builder_reduce_with": (c_u32, [c_p, c_u32, c_u32, c_u32, P(c_str), c_u32, P(c_u32)]),
     "accy_b200_builder_mean": (c_u32, [c_p, c_u32, P(c_str), c_u32, P(c_u32)]),
     "accy_b200_builder_contract": (c_u32, [c_p, c_u32, c_u32, P(c_str), c_u32, P(c_u32)]),
+    "accy_b200_builder_gather": (c_u32, [c_p, c_u32, c_u32, c_str, P(c_u32)]),
+    "accy_b200_builder_scatter_add": (c_u32, [c_p, c_u32, c_u32, c_u32, c_str, P(c_u32)]),
+    "accy_b200_builder_token_log_prob": (c_u32, [c_p, c_u32, c_u32, c_str, P(c_u32)]),
     "accy_b200_builder_rename": (c_u32, [c_p, c_u32, c_str, c_str, P(c_u32)]),
     "accy_b200_builder_split": (c_u32, [c_p, c_u32, c_str, P(c_str), P(ctypes.c_int64), c_u32, P(c_u32)]),
     "accy_b200_builder_merge": (c_u32, [c_p, c_u32, P(c_str), c_u32, c_str, P(c_u32)]),

@@ -15,7 +15,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaccy_b200.so")
-SOURCES = ["program.cpp", "wire.cpp", "planner.cpp", "emit_row.cpp", "emit_gemm.cpp", "emit_tc.cpp", "emit_attn.cpp", "shard.cpp", "transform.cpp",
+SOURCES = ["program.cpp", "wire.cpp", "planner.cpp", "emit_row.cpp", "emit_gemm.cpp", "emit_tc.cpp", "emit_attn.cpp", "emit_token.cpp", "shard.cpp", "transform.cpp",
            "driver.cpp", "session.cpp", "sharded.cpp"]
 
 

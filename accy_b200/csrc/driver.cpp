@@ -68,6 +68,7 @@ void loadReal() {
   bind(lib, g_real.cuGraphLaunch, "cuGraphLaunch");
   bind(lib, g_real.cuGraphExecDestroy, "cuGraphExecDestroy");
   bind(lib, g_real.cuGraphDestroy, "cuGraphDestroy");
+  bind(lib, g_real.cuStreamIsCapturing, "cuStreamIsCapturing");
   CUresult_t r = g_real.cuInit(0);
   if (r != 0) throw std::runtime_error("cuInit failed: " + std::to_string(r));
   g_real_loaded = true;
@@ -159,6 +160,10 @@ CUresult_t f_cuGraphInstantiateWithFlags(CUgraphExec_t* e, CUgraph_t, unsigned l
 CUresult_t f_cuGraphLaunch(CUgraphExec_t, CUstream_t) { return fakeResult("cuGraphLaunch"); }
 CUresult_t f_cuGraphExecDestroy(CUgraphExec_t) { return fakeResult("cuGraphExecDestroy"); }
 CUresult_t f_cuGraphDestroy(CUgraph_t) { return fakeResult("cuGraphDestroy"); }
+CUresult_t f_cuStreamIsCapturing(CUstream_t, int* status) {
+  *status = 0;
+  return fakeResult("cuStreamIsCapturing");
+}
 
 const DriverTable g_fake = {
     f_cuInit, f_cuDeviceGet, f_cuDeviceGetCount, f_cuDeviceGetAttribute, f_cuDevicePrimaryCtxRetain,
@@ -168,7 +173,7 @@ const DriverTable g_fake = {
     f_cuStreamSynchronize, f_cuStreamWaitEvent, f_cuEventCreate, f_cuEventDestroy, f_cuEventRecord,
     f_cuEventSynchronize, f_cuEventElapsedTime, f_cuGetErrorName, f_cuTensorMapEncodeTiled,
     f_cuStreamBeginCapture, f_cuStreamEndCapture, f_cuGraphInstantiateWithFlags, f_cuGraphLaunch,
-    f_cuGraphExecDestroy, f_cuGraphDestroy};
+    f_cuGraphExecDestroy, f_cuGraphDestroy, f_cuStreamIsCapturing};
 
 // ---- NVRTC ----
 struct Nvrtc {

@@ -69,6 +69,7 @@ struct DriverTable {
   CUresult_t (*cuGraphLaunch)(CUgraphExec_t, CUstream_t);
   CUresult_t (*cuGraphExecDestroy)(CUgraphExec_t);
   CUresult_t (*cuGraphDestroy)(CUgraph_t);
+  CUresult_t (*cuStreamIsCapturing)(CUstream_t, int* status);
 };
 
 // Returns the active table: the real driver (loaded on first call) or the fake.  Throws

@@ -216,7 +216,7 @@ __device__ __forceinline__ T group_reduce(T v, T* cells, int t, int rsub) {
 }
 )CUDA";
 
-namespace {
+const char* kernelPrelude() { return kRowPrelude; }
 
 // index expression for dims [lo, hi) addressed by the flat index `flat` (row-major over those
 // dims): adjacent dims whose strides chain are merged so that contiguous buffers cost one multiply
@@ -252,6 +252,8 @@ std::string indexExpr(const std::vector<int64_t>& extents, const std::vector<int
   }
   return any ? out.str() : std::string("0ll");
 }
+
+namespace {
 
 struct RowGen {
   const Cluster& c;
@@ -320,15 +322,35 @@ struct RowGen {
     return true;
   }
 
+  // Declares `var`: the offset that a looked-up leaf's index adds here, or -1 where the index is outside
+  // the axis.  `col` is the flat column, "" where the index does not vary along the columns.
+  void emitLookup(int leaf, const std::string& var, const std::string& col, const std::string& indent) {
+    const LeafRef& l = c.leaves[leaf];
+    const LeafRef& ix = c.leaves[l.index_leaf];
+    std::string at = indexExpr(c.extents, ix.strides, 0, c.split, rowVar());
+    if (!col.empty()) at += " + " + indexExpr(c.extents, ix.strides, c.split, static_cast<int>(c.extents.size()), col);
+    o << indent << "long long " << var << " = (long long)L" << l.index_leaf << "[" << at << "];\n";
+    o << indent << var << " = " << var << " >= 0 && " << var << " < " << l.index_extent << "ll ? " << var << " * "
+      << l.index_stride << "ll : -1ll;\n";
+  }
+  // whether a looked-up leaf takes a number per element instead of one per row
+  bool indexedByElement(const LeafRef& l) const { return l.index_leaf >= 0 && (c.leaves[l.index_leaf].vary & ~row_mask) != 0; }
+
   // ---- scalar (S / R class) nodes ----
   void emitScalarNode(int i, const std::string& indent, const std::vector<std::string>* red_values) {
     const ENode& n = c.nodes[i];
     const std::string ty = ctypeOf(n.dtype);
+    if (n.op == ENode::Leaf && c.leaves[n.leaf].index_leaf >= 0) emitLookup(n.leaf, "gi_" + name(i), "", indent);
     o << indent << "const " << ty << " " << name(i) << " = ";
     switch (n.op) {
       case ENode::Leaf: {
         const LeafRef& l = c.leaves[n.leaf];
         std::string off = indexExpr(c.extents, l.strides, 0, c.split, rowVar());
+        if (l.index_leaf >= 0) {
+          const std::string gi = "gi_" + name(i);
+          o << "(" << gi << " < 0 ? (" << ty << ")0 : " << loadConvert(l.dtype, "L" + std::to_string(n.leaf) + "[" + off + " + " + gi + "]") << ")";
+          break;
+        }
         o << loadConvert(l.dtype, "L" + std::to_string(n.leaf) + "[" + off + "]");
         break;
       }
@@ -391,12 +413,25 @@ struct RowGen {
       const std::string L = "L" + std::to_string(n.leaf);
       const std::string st = storageTypeOf(l.dtype);
       std::string rowoff = indexExpr(c.extents, l.strides, 0, c.split, rowVar());
-      o << indent << "{\n" << indent << "  const long long ro = " << rowoff << ";\n";
+      const bool lookup = l.index_leaf >= 0, by_element = indexedByElement(l);
+      o << indent << "{\n";
+      if (lookup && !by_element) {
+        emitLookup(n.leaf, "gi", "", indent + "  ");
+        rowoff += " + gi";
+      }
+      o << indent << "  const long long ro = " << rowoff << ";\n";
       o << indent << "#pragma unroll\n" << indent << "  for (int j = 0; j < " << s.vpt << "; ++j) {\n";
       o << indent << "    const long long c0 = cb + (long long)(j * " << s.tpr << " + t) * " << s.vec << ";\n";
-      if (colContiguous(l)) {
+      if (by_element) {
+        std::string coloff = indexExpr(c.extents, l.strides, c.split, static_cast<int>(c.extents.size()), "c0");
+        o << indent << "    " << st << " raw = 0;\n" << indent << "    if (" << (always_valid ? "true" : "c0 < cend") << ") {\n";
+        emitLookup(n.leaf, "gi", "c0", indent + "      ");
+        o << indent << "      if (gi >= 0) raw = " << L << "[ro + gi + " << coloff << "];\n" << indent << "    }\n";
+        o << indent << "    " << name(i) << "[j] = " << loadConvert(l.dtype, "raw") << ";\n";
+      } else if (colContiguous(l)) {
         o << indent << "    Pack<" << st << ", " << s.vec << "> p;\n";
-        o << indent << "    if (" << (always_valid ? "true" : "c0 < cend") << ") p = *reinterpret_cast<const Pack<" << st
+        const std::string valid = std::string(always_valid ? "true" : "c0 < cend") + (lookup ? " && gi >= 0" : "");
+        o << indent << "    if (" << valid << ") p = *reinterpret_cast<const Pack<" << st
           << ", " << s.vec << ">*>(" << L << " + ro + c0);\n";
         o << indent << "    else {\n" << indent << "#pragma unroll\n" << indent << "      for (int e = 0; e < "
           << s.vec << "; ++e) p.v[e] = 0; }\n";
@@ -404,8 +439,9 @@ struct RowGen {
           << "[j * " << s.vec << " + e] = " << loadConvert(l.dtype, "p.v[e]") << ";\n";
       } else {
         std::string coloff = indexExpr(c.extents, l.strides, c.split, static_cast<int>(c.extents.size()), "c0");
+        const std::string valid = std::string(always_valid ? "true" : "c0 < cend") + (lookup ? " && gi >= 0" : "");
         o << indent << "    " << st << " raw = 0;\n";
-        o << indent << "    if (" << (always_valid ? "true" : "c0 < cend") << ") raw = " << L << "[ro + " << coloff << "];\n";
+        o << indent << "    if (" << valid << ") raw = " << L << "[ro + " << coloff << "];\n";
         o << indent << "    " << name(i) << "[j] = " << loadConvert(l.dtype, "raw") << ";\n";
       }
       o << indent << "  }\n" << indent << "}\n";
@@ -1213,6 +1249,7 @@ RowSchedule chooseRowSchedule(const Cluster& c, const ScheduleOverrides& o) {
   for (size_t l = 0; l < c.leaves.size(); ++l) {
     const LeafRef& leaf = c.leaves[l];
     if ((leaf.vary & ~row_mask) == 0) continue;  // read once per row as a scalar
+    if (leaf.index_leaf >= 0 && (c.leaves[leaf.index_leaf].vary & ~row_mask) != 0) gather = true;  // a number per element
     int es = static_cast<int>(dtypeSize(leaf.dtype));
     vec = std::min(vec, std::max(1, 16 / es));
     int64_t expect = 1;
@@ -1226,6 +1263,7 @@ RowSchedule chooseRowSchedule(const Cluster& c, const ScheduleOverrides& o) {
   auto rowsAligned = [&](int v) {
     for (const LeafRef& leaf : c.leaves) {
       if ((leaf.vary & ~row_mask) == 0) continue;
+      if (leaf.index_leaf >= 0 && leaf.index_stride % v != 0) return false;
       for (int d = 0; d < c.split; ++d)
         if (c.extents[d] != 1 && leaf.strides[d] % v != 0) return false;
     }

@@ -12,6 +12,9 @@
 //     and its row pipeline, row.zig:556-668, without their op-count and column limits);
 //   * a dot_general plus the elementwise ops that only it feeds becomes one GEMM with an epilogue
 //     (fusion/pass.zig:1585-1699, without the 6-op chain limit);
+//   * a gather is index arithmetic of the kernel that consumes it (an indirect row offset); a
+//     scatter_add takes the elementwise ops that compute its updates; a token's log-probability and
+//     its gradient become one kernel together with the per-row ops between them;
 //   * dot -> scale -> [causal mask] -> softmax -> dot becomes one attention kernel
 //     (fusion/pass.zig:729-905, extended to causal masks, batch axes and bf16).
 // Anything else is refused at compile time; there is no CPU fallback.
@@ -42,7 +45,11 @@ struct LeafRef {
   int slot = -1;                  // plan slot holding the buffer
   DType dtype = DType::f32;
   std::vector<int64_t> strides;   // element stride per cluster dim (0 = broadcast)
-  uint32_t vary = 0;
+  uint32_t vary = 0;              // dims its value changes along (those of the index leaf included)
+  // A looked-up buffer (gather): the element also moves by index_stride times the number another leaf
+  // holds here, and reads as zero where that number is outside [0, index_extent).
+  int index_leaf = -1;            // index into the same list of leaves
+  int64_t index_stride = 0, index_extent = 0;
 };
 
 struct ClusterOutput {
@@ -89,6 +96,32 @@ struct AttentionOp {
   float scale = 1.0f;
   bool causal = false;
   DType dtype = DType::bf16;
+};
+
+// out = base + the updates summed into the rows that `indices` numbers, over [pre, axis, post].
+struct ScatterOp {
+  int64_t pre = 1, extent = 0, post = 1, count = 0;   // count: how many indices
+  int base_slot = -1;             // -1: zeros
+  int index_slot = -1, out_slot = -1;
+  DType dtype = DType::f32, base_dtype = DType::f32, index_dtype = DType::i32, out_dtype = DType::f32;  // value type; storage types
+  // The updates as an expression over [pre, indices..., post...]: rows (pre and indices) below `split`.
+  Cluster updates;
+  int result = -1;                // node of `updates` that is summed
+};
+
+// Log-probabilities of one token per row of [rows, vocab] and / or their gradient with respect to the
+// logits, scaled by a slope per row.
+struct TokenOp {
+  int64_t rows = 1, vocab = 0;
+  std::vector<int64_t> row_extents;
+  int logits_slot = -1, token_slot = -1;
+  DType logits_dtype = DType::f32, token_dtype = DType::i32;   // storage types
+  int log_prob_slot = -1;         // written when >= 0
+  int stats_out = -1, stats_in = -1;  // (row maximum, sum of exponentials) written / read in place of a pass
+  int grad_slot = -1;             // written when >= 0
+  DType grad_dtype = DType::f32;
+  // The slope as an expression over the row dims; node `acc` stands for the row's log-probability.
+  Epilogue slope;
 };
 
 struct Slot {
@@ -200,6 +233,12 @@ void emitRowKernels(const Cluster& c, const RowSchedule& s, const std::string& n
 void emitGemm(const GemmOp& g, const std::string& name, Plan& plan, const ScheduleOverrides& o);
 void emitAttention(const AttentionOp& a, const std::string& name, Plan& plan,
                    const ScheduleOverrides& o);
+void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, const ScheduleOverrides& o);
+void emitTokenLogProb(const TokenOp& t, const std::string& name, Plan& plan, const ScheduleOverrides& o);
+// C expression of the element offset that flat index `flat` over dims [lo, hi) has under `strides`.
+std::string indexExpr(const std::vector<int64_t>& extents, const std::vector<int64_t>& strides, int lo, int hi,
+                      const std::string& flat);
+const char* kernelPrelude();   // conversions, packed arithmetic and row reductions shared by generated kernels
 // Emits the C expression that evaluates an elementwise node from its operand expressions.
 std::string elementwiseExpr(const ENode& n, const std::string& a, const std::string& b,
                             const std::string& c, DType a_dtype);

@@ -224,6 +224,12 @@ class Planner {
         if (tryAttention(v)) return slot_of[v];
         planGemm(v, v);
         return slot_of[v];
+      case Kind::scatter_add:
+        planScatterAdd(v);
+        return slot_of[v];
+      case Kind::custom_call:
+        planTokens(v);
+        return slot_of[v];
       default:
         break;
     }
@@ -267,7 +273,7 @@ class Planner {
     return static_cast<int>(b.nodes.size()) - 1;
   }
 
-  int leafNode(Build& b, int slot, const Type& ty, const std::vector<int>& map) {
+  int leafNode(Build& b, int slot, const Type& ty, const std::vector<int>& map, int index_leaf = -1, int64_t index_axis = 0) {
     LeafRef leaf;
     leaf.slot = slot;
     leaf.dtype = plan.slots[slot].storage;
@@ -278,10 +284,16 @@ class Planner {
       leaf.strides[map[i]] += rm[i];
       leaf.vary |= 1u << map[i];
     }
+    if (index_leaf >= 0) {
+      leaf.index_leaf = index_leaf;
+      leaf.index_stride = rm[index_axis];
+      leaf.index_extent = ty.dims[index_axis].extent;
+      leaf.vary |= b.leaves[index_leaf].vary;
+    }
     // leaves are deduplicated so one buffer read with one index map is loaded once
     int index = -1;
     for (size_t i = 0; i < b.leaves.size(); ++i) {
-      if (b.leaves[i].slot == slot && b.leaves[i].strides.size() <= leaf.strides.size()) {
+      if (b.leaves[i].slot == slot && b.leaves[i].index_leaf == leaf.index_leaf && b.leaves[i].index_stride == leaf.index_stride && b.leaves[i].strides.size() <= leaf.strides.size()) {
         bool same = true;
         for (size_t d = 0; d < leaf.strides.size(); ++d) {
           int64_t have = d < b.leaves[i].strides.size() ? b.leaves[i].strides[d] : 0;
@@ -346,7 +358,7 @@ class Planner {
 
   int buildNodeUncached(Build& b, uint32_t v, const std::vector<int>& map) {
     const Operation& op = P.ops[v];
-    if (b.trial && v == b.acc_value) {
+    if (b.trial && (v == b.acc_value || (op.kind == Kind::custom_call && sameValue(v, b.acc_value)))) {
       for (size_t i = 0; i < map.size(); ++i)
         if (map[i] != static_cast<int>(i)) throw Abort{};
       if (b.acc_node < 0) {
@@ -453,7 +465,22 @@ class Planner {
       case Kind::reduce:
         return buildReduce(b, v, map);
       case Kind::dot_general:
+      case Kind::scatter_add:
+      case Kind::custom_call:
         return boundaryLeaf(b, v, map);
+      case Kind::gather: {
+        // rows read through an index: an indirect offset in whatever kernel this region becomes
+        if (b.trial) throw Abort{};  // GEMM epilogues take no lookups
+        const uint32_t data = op.operands[0], indices = op.operands[1];
+        const Type &dt = P.typeOf(data), &it = P.typeOf(indices);
+        std::vector<int> data_map, index_map(map.begin() + op.axis, map.begin() + op.axis + static_cast<long>(it.rank()));
+        for (size_t i = 0; i < dt.rank(); ++i)
+          data_map.push_back(static_cast<int64_t>(i) < op.axis ? map[i] : static_cast<int64_t>(i) == op.axis ? -1 : map[i - 1 + it.rank()]);
+        materialize(data);
+        materialize(indices);
+        const ENode number = b.nodes[leafNode(b, slot_of[indices], it, index_map)];
+        return leafNode(b, slot_of[data], dt, data_map, number.leaf, op.axis);
+      }
       default:
         throw PlanError(std::string("operation kind not supported by the B200 target: ") + kindName(op.kind));
     }
@@ -554,7 +581,12 @@ class Planner {
   // ---------------------------------------------------------------------------------------
   // row kernels
   // ---------------------------------------------------------------------------------------
-  int cluster_depth = 0;  // nesting of planCluster calls (a region materialising what it reads)
+  int cluster_depth = 0;  // nesting of regions being planned (a region materialising what it reads)
+  struct Depth {
+    int& d;
+    explicit Depth(int& v) : d(v) { ++d; }
+    ~Depth() { --d; }
+  };
 
   void planCluster(uint32_t v) {
     if (!is_output[v]) standalone.insert(same_as[v]);
@@ -568,11 +600,7 @@ class Planner {
       b.is_col.push_back(false);
       map[i] = static_cast<int>(i);
     }
-    struct Depth {
-      int& d;
-      explicit Depth(int& v) : d(v) { ++d; }
-      ~Depth() { --d; }
-    } depth(cluster_depth);
+    Depth depth(cluster_depth);
     int root_node = buildNode(b, v, map);
     // Sibling outputs with the root's own dims (e.g. a value and its slope, both sums over the
     // same axis) join this region, so inputs they share are read once (the reference's concat
@@ -628,8 +656,11 @@ class Planner {
         b.is_col.push_back(true);
       } else {
         int64_t cols = 1;
+        uint32_t numbered = 0;   // dims that looked-up rows are numbered along: columns stop before them
+        for (const LeafRef& leaf : b.leaves)
+          if (leaf.index_leaf >= 0) numbered |= b.leaves[leaf.index_leaf].vary;
         for (long d = static_cast<long>(b.extents.size()) - 1; d >= 0; --d) {
-          if (cols >= 1024) break;
+          if (cols >= 1024 || (cols > 1 && (numbered & (1u << d)))) break;
           b.is_col[d] = true;
           cols *= b.extents[d];
         }
@@ -1045,6 +1076,219 @@ class Planner {
   }
 
   // ---------------------------------------------------------------------------------------
+  // scatter_add
+  // ---------------------------------------------------------------------------------------
+  bool isZeros(uint32_t v) {
+    double c;
+    return scalarConstant(v, &c) && c == 0.0;
+  }
+
+  void planScatterAdd(uint32_t v) {
+    Depth depth(cluster_depth);
+    const Operation& op = P.ops[v];
+    const uint32_t base = op.operands[0], indices = op.operands[1], updates = op.operands[2];
+    const Type &bt = op.result, &it = P.typeOf(indices), &ut = P.typeOf(updates);
+    ScatterOp s;
+    s.dtype = bt.dtype;
+    for (size_t i = 0; i < bt.rank(); ++i)
+      (static_cast<int64_t>(i) < op.axis ? s.pre : static_cast<int64_t>(i) == op.axis ? s.extent : s.post) =
+          static_cast<int64_t>(i) == op.axis ? bt.dims[i].extent
+                                             : (static_cast<int64_t>(i) < op.axis ? s.pre : s.post) * bt.dims[i].extent;
+    s.count = static_cast<int64_t>(it.elementCount());
+    materialize(indices);
+    s.index_slot = slot_of[indices];
+    s.index_dtype = plan.slots[s.index_slot].storage;
+    if (!isZeros(base)) {
+      s.base_slot = materialize(base);
+      s.base_dtype = plan.slots[s.base_slot].storage;
+    }
+    // The updates: the elementwise ops that compute them are evaluated where they are summed, unless
+    // another kernel needs them too or they are not elementwise all the way.
+    Build b;
+    b.root = updates;
+    std::vector<int> map(ut.rank());
+    auto fresh = [&] {
+      b = Build{};
+      b.root = updates;
+      for (size_t i = 0; i < ut.rank(); ++i) {
+        b.dim_names.push_back(ut.dims[i].name);
+        b.extents.push_back(ut.dims[i].extent);
+        b.is_col.push_back(i >= static_cast<size_t>(op.axis) + it.rank());
+        map[i] = static_cast<int>(i);
+      }
+    };
+    fresh();
+    materializeFolds(updates);
+    b.trial = true;
+    try {
+      s.result = buildNode(b, updates, map);
+    } catch (const Abort&) {
+      fresh();
+      materialize(updates);
+      s.result = leafNode(b, slot_of[updates], ut, map);
+    }
+    s.updates.split = static_cast<int>(op.axis + static_cast<int64_t>(it.rank()));
+    s.updates.extents = b.extents;
+    for (size_t i = 0; i < b.extents.size(); ++i) (static_cast<int>(i) < s.updates.split ? s.updates.rows : s.updates.cols) *= b.extents[i];
+    s.updates.nodes = b.nodes;
+    s.updates.leaves = b.leaves;
+    s.out_slot = destinationSlot(v);
+    s.out_dtype = plan.slots[s.out_slot].storage;
+    const std::string name = nextName("scatter");
+    summary << "scatter_add: " << name << " pre=" << s.pre << " rows=" << s.extent << " cols=" << s.post << " indices=" << s.count
+            << " nodes=" << b.nodes.size() << (s.base_slot < 0 ? " from zeros" : " on a base") << "\n";
+    emitScatterAdd(s, name, plan, ov);
+    slot_of[v] = s.out_slot;
+    produced.insert(v);
+  }
+
+  // Gives every fold, contraction, lookup and call that `v` is computed from elementwise (through
+  // broadcasts, transposes and relabelling reshapes) a buffer, stopping at `except`.  What is left
+  // between those buffers and `v` can then be evaluated inside another kernel.
+  void materializeFolds(uint32_t v, uint32_t except = kNone) {
+    const Operation& op = P.ops[v];
+    if (sameValue(v, except) || slot_of[v] >= 0 || op.kind == Kind::constant || op.kind == Kind::iota) return;
+    if (isElementwise(op.kind) || op.kind == Kind::broadcast_in_dim || op.kind == Kind::transpose || op.kind == Kind::reshape) {
+      for (uint32_t a : op.operands) materializeFolds(a, except);
+      return;
+    }
+    materialize(v);
+  }
+
+  // ---------------------------------------------------------------------------------------
+  // log-probabilities of tokens, and their gradient
+  // ---------------------------------------------------------------------------------------
+  static constexpr uint32_t kNone = 0xffffffffu;
+  std::map<uint32_t, int> stats_of;   // log-probability op -> slot with its rows' maxima and sums
+
+  // the call of the given kind on the same logits and tokens as `v` that something needs
+  uint32_t partnerOf(uint32_t v, Call want) {
+    for (const Operation& op : P.ops) {
+      if (op.kind != Kind::custom_call || op.sub != static_cast<uint8_t>(want) || same_as[op.id] != op.id) continue;
+      if (same_as[op.operands[0]] != same_as[P.ops[v].operands[0]] || same_as[op.operands[1]] != same_as[P.ops[v].operands[1]]) continue;
+      if (is_output[op.id] || !users[op.id].empty()) return op.id;
+    }
+    return kNone;
+  }
+
+  // one value under one or two names (kNone is no value's)
+  bool sameValue(uint32_t a, uint32_t b) const { return a == b || (a != kNone && b != kNone && same_as[a] == same_as[b]); }
+
+  bool dependsOn(uint32_t v, uint32_t on, std::set<uint32_t>& seen) {
+    if (sameValue(v, on)) return true;
+    if (!seen.insert(v).second) return false;
+    for (uint32_t a : P.ops[v].operands)
+      if (dependsOn(a, on, seen)) return true;
+    return false;
+  }
+  bool dependsOn(uint32_t v, uint32_t on) {
+    std::set<uint32_t> seen;
+    return dependsOn(v, on, seen);
+  }
+
+  // whether `v` is computed from `from` by elementwise operations and views alone
+  bool elementwiseFrom(uint32_t v, uint32_t from) {
+    if (sameValue(v, from) || !dependsOn(v, from)) return true;
+    const Operation& op = P.ops[v];
+    if (!isElementwise(op.kind) && op.kind != Kind::broadcast_in_dim && op.kind != Kind::transpose && op.kind != Kind::reshape) return false;
+    for (uint32_t a : op.operands)
+      if (!elementwiseFrom(a, from)) return false;
+    return true;
+  }
+
+  // The slope of a gradient as an expression over its rows, with `log_prob` (if any) standing for the
+  // kernel's own log-probability; false where that value is seen in another order.
+  bool slopeOf(uint32_t slope, uint32_t log_prob, Epilogue* out) {
+    const Type& ty = P.typeOf(slope);
+    Build b;
+    std::vector<int> map(ty.rank());
+    b.root = slope;
+    b.trial = true;
+    b.acc_value = log_prob;
+    for (size_t i = 0; i < ty.rank(); ++i) {
+      b.dim_names.push_back(ty.dims[i].name);
+      b.extents.push_back(ty.dims[i].extent);
+      b.is_col.push_back(false);
+      map[i] = static_cast<int>(i);
+    }
+    materializeFolds(slope, log_prob);
+    try {
+      out->result = buildNode(b, slope, map);
+    } catch (const Abort&) {
+      return false;
+    }
+    out->nodes = b.nodes;
+    out->leaves = b.leaves;
+    out->acc = b.acc_node;
+    return true;
+  }
+
+  void planTokens(uint32_t v) {
+    Depth depth(cluster_depth);
+    const bool is_grad = static_cast<Call>(P.ops[v].sub) == Call::token_log_prob_grad;
+    uint32_t forward = is_grad ? partnerOf(v, Call::token_log_prob) : v;
+    uint32_t grad = is_grad ? v : partnerOf(v, Call::token_log_prob_grad);
+    auto open = [&](uint32_t x) { return x != kNone && slot_of[x] < 0 && !produced.count(x); };
+    TokenOp t;
+    const Operation& any = P.ops[v];
+    const Type &lt = P.typeOf(any.operands[0]), &kt = P.typeOf(any.operands[1]);
+    t.vocab = lt.dims.back().extent;
+    t.rows = static_cast<int64_t>(kt.elementCount());
+    for (const Dim& d : kt.dims) t.row_extents.push_back(d.extent);
+    t.logits_slot = materialize(any.operands[0]);
+    t.token_slot = materialize(any.operands[1]);
+    t.logits_dtype = plan.slots[t.logits_slot].storage;
+    t.token_dtype = plan.slots[t.token_slot].storage;
+    const bool both = open(forward) && open(grad) && elementwiseFrom(P.ops[grad].operands[2], forward) &&
+                      slopeOf(P.ops[grad].operands[2], forward, &t.slope);
+    if (!both && is_grad) {
+      // the slope needs log-probabilities of other rows: they come first, in a kernel of their own,
+      // which leaves its rows' maxima and sums for this one
+      materializeFolds(any.operands[2]);
+      if (slot_of[v] >= 0) return;
+      forward = kNone;
+      t.slope = Epilogue{};
+      if (!slopeOf(any.operands[2], kNone, &t.slope)) {
+        materialize(any.operands[2]);
+        t.slope = Epilogue{};
+        if (!slopeOf(any.operands[2], kNone, &t.slope)) throw PlanError("internal: slope of a token gradient");
+      }
+      const uint32_t first = partnerOf(v, Call::token_log_prob);
+      auto stats = first == kNone ? stats_of.end() : stats_of.find(first);
+      if (stats != stats_of.end()) t.stats_in = stats->second;
+    }
+    if (!both && !is_grad) {
+      if (open(grad)) {
+        t.stats_out = newSlot(Slot::Temp, static_cast<size_t>(t.rows) * 8, v, DType::f32);
+        stats_of[v] = t.stats_out;
+      }
+      grad = kNone;
+    }
+    if (forward != kNone && open(forward)) {
+      t.log_prob_slot = destinationSlot(forward);
+    } else {
+      forward = kNone;
+    }
+    if (grad != kNone) {
+      t.grad_slot = destinationSlot(grad);
+      t.grad_dtype = plan.slots[t.grad_slot].storage;
+    }
+    const std::string name = nextName("tokens");
+    summary << "token log-probabilities: " << name << " rows=" << t.rows << " vocab=" << t.vocab << " logits=" << dtypeName(t.logits_dtype)
+            << (forward != kNone ? " value" : "") << (grad != kNone ? " gradient" : "") << (t.stats_in >= 0 ? " from kept sums" : "") << "\n";
+    emitTokenLogProb(t, name, plan, ov);
+    plan.work.pairs += static_cast<double>(t.rows) * static_cast<double>(t.vocab);
+    if (forward != kNone) {
+      slot_of[forward] = t.log_prob_slot;
+      produced.insert(forward);
+    }
+    if (grad != kNone) {
+      slot_of[grad] = t.grad_slot;
+      produced.insert(grad);
+    }
+  }
+
+  // ---------------------------------------------------------------------------------------
   // attention
   // ---------------------------------------------------------------------------------------
   uint32_t throughBroadcast(uint32_t v, std::vector<int64_t>* bd = nullptr) {
@@ -1254,6 +1498,11 @@ static bool foldsInTwoStages(const Program& p, const Operation& op) {
   return inner_reduced && other_reduced;
 }
 
+static uint32_t zerosOf(Builder& b, const Type& ty) {
+  const std::vector<uint8_t> zero(dtypeSize(ty.dtype), 0);
+  return b.broadcastTo(b.constantBytes(Type{ty.dtype, {}}, zero.data(), zero.size()), ty.dims, {});
+}
+
 static Program withoutEmptyFolds(const Program& p) {
   Builder b(p.name);
   std::vector<uint32_t> now(p.ops.size(), 0);
@@ -1331,6 +1580,35 @@ static Program withoutEmptyFolds(const Program& p) {
           made = b.dotGeneralOp(lhs, rhs, lhs_contract, rhs_contract, batch_axes, batch_axes);
         }
         break;
+      case Kind::gather:
+        if (!empty && p.typeOf(op.operands[0]).elementCount() == 0) made = zerosOf(b, op.result);  // no row to read
+        else made = b.gather(arg(0), arg(1), op.axis);
+        break;
+      case Kind::scatter_add:
+        if (p.typeOf(op.operands[2]).elementCount() == 0) made = arg(0);  // nothing to add
+        else made = b.scatterAdd(arg(0), arg(1), arg(2), op.axis);
+        break;
+      case Kind::custom_call: {
+        const Type& logits = p.typeOf(op.operands[0]);
+        if (logits.elementCount() == 0) {   // no token is in an empty vocabulary
+          made = zerosOf(b, op.result);
+          break;
+        }
+        // the vocabulary is brought to the end by a transpose, and the gradient back
+        const size_t axis = vocabularyAxis(logits.dims, p.typeOf(op.operands[1]).dims);
+        std::vector<int64_t> perm, inverse(logits.rank());
+        for (size_t i = 0; i < logits.rank(); ++i)
+          if (i != axis) perm.push_back(static_cast<int64_t>(i));
+        perm.push_back(static_cast<int64_t>(axis));
+        for (size_t i = 0; i < perm.size(); ++i) inverse[perm[i]] = static_cast<int64_t>(i);
+        const bool last = axis + 1 == logits.rank();
+        std::vector<uint32_t> operands;
+        for (size_t i = 0; i < op.operands.size(); ++i) operands.push_back(arg(i));
+        if (!last) operands[0] = b.transposeBy(operands[0], perm);
+        made = b.customCall(static_cast<Call>(op.sub), operands);
+        if (!last && static_cast<Call>(op.sub) == Call::token_log_prob_grad) made = b.transposeBy(made, inverse);
+        break;
+      }
       default:
         throw PlanError("operation kind not supported by the B200 target");
     }
@@ -1352,6 +1630,10 @@ Plan planProgram(const Program& program, const ScheduleOverrides& overrides) {
   for (const Operation& op : program.ops) {
     reorder |= op.kind == Kind::broadcast;
     reorder |= op.kind == Kind::reduce && foldsInTwoStages(program, op);
+    if (op.kind == Kind::custom_call) {
+      const Type& logits = program.typeOf(op.operands[0]);
+      reorder |= vocabularyAxis(logits.dims, program.typeOf(op.operands[1]).dims) + 1 != logits.rank();
+    }
     if (op.kind != Kind::dot_general) continue;
     const size_t nb = op.lhs_batch.size(), nk = op.ints.size();
     const size_t nm = program.typeOf(op.operands[0]).rank() - nb - nk;

@@ -35,6 +35,22 @@ bool dtypeIsFloat(DType d) {
   return d == DType::f16 || d == DType::bf16 || d == DType::f32 || d == DType::f64;
 }
 
+bool dtypeIsIndex(DType d) { return d >= DType::i8 && d <= DType::u64; }
+
+const char* callTarget(Call c) {
+  static const char* names[] = {"accy_b200.token_log_prob", "accy_b200.token_log_prob_grad"};
+  return names[static_cast<int>(c)];
+}
+
+bool customCallOf(const std::string& target, uint32_t version, Call* call) {
+  for (uint32_t i = 0; i < kCallCount; ++i) {
+    if (version != 1 || target != callTarget(static_cast<Call>(i))) continue;
+    *call = static_cast<Call>(i);
+    return true;
+  }
+  return false;
+}
+
 const char* kindName(Kind k) {
   static const char* names[] = {"parameter", "constant", "unary", "binary", "iota", "broadcast",
                                 "broadcast_in_dim", "reshape", "transpose", "reduce", "gather",
@@ -457,6 +473,101 @@ uint32_t Builder::alignedSelect(uint32_t pred, uint32_t on_true, uint32_t on_fal
   uint32_t f = alignTo(on_false, target);
   uint32_t p = scalar_pred ? pred : alignTo(pred, target);
   return select(p, t, f);
+}
+
+std::vector<Dim> replacedAxis(const std::vector<Dim>& dims, int64_t axis, const std::vector<Dim>& by) {
+  validateAxes(dims.size(), {axis});
+  std::vector<Dim> out(dims.begin(), dims.begin() + axis);
+  out.insert(out.end(), by.begin(), by.end());
+  out.insert(out.end(), dims.begin() + axis + 1, dims.end());
+  validateDims(out);
+  return out;
+}
+
+size_t vocabularyAxis(const std::vector<Dim>& logits, const std::vector<Dim>& tokens) {
+  if (logits.size() != tokens.size() + 1) throw TensorError("RankMismatch");
+  size_t axis = 0;
+  while (axis < tokens.size() && logits[axis].name == tokens[axis].name) ++axis;
+  std::vector<Dim> rest = logits;
+  rest.erase(rest.begin() + static_cast<long>(axis));
+  if (!sameDims(rest, tokens)) throw TensorError("ShapeMismatch");
+  return axis;
+}
+
+uint32_t Builder::gather(uint32_t data, uint32_t indices, int64_t axis) {
+  ensure(data);
+  ensure(indices);
+  if (!dtypeIsIndex(typeOf(indices).dtype)) throw TensorError("NonIntegerDType");
+  Operation op;
+  op.kind = Kind::gather;
+  op.operands = {data, indices};
+  op.axis = axis;
+  op.result = Type{typeOf(data).dtype, replacedAxis(typeOf(data).dims, axis, typeOf(indices).dims)};
+  return emit(std::move(op));
+}
+
+uint32_t Builder::scatterAdd(uint32_t base, uint32_t indices, uint32_t updates, int64_t axis) {
+  ensure(base);
+  ensure(indices);
+  ensure(updates);
+  if (!dtypeIsIndex(typeOf(indices).dtype)) throw TensorError("NonIntegerDType");
+  if (!dtypeIsFloat(typeOf(base).dtype)) throw TensorError("NonFloatDType");
+  if (typeOf(base).dtype != typeOf(updates).dtype) throw TensorError("DTypeMismatch");
+  if (!sameDims(typeOf(updates).dims, replacedAxis(typeOf(base).dims, axis, typeOf(indices).dims)))
+    throw TensorError("ShapeMismatch");
+  Operation op;
+  op.kind = Kind::scatter_add;
+  op.operands = {base, indices, updates};
+  op.axis = axis;
+  op.result = typeOf(base);
+  return emit(std::move(op));
+}
+
+uint32_t Builder::customCall(Call call, const std::vector<uint32_t>& operands) {
+  for (uint32_t id : operands) ensure(id);
+  if (operands.size() != (call == Call::token_log_prob ? 2u : 3u)) throw TensorError("OperandCountMismatch");
+  const Type logits = typeOf(operands[0]), tokens = typeOf(operands[1]);
+  if (!dtypeIsFloat(logits.dtype) || logits.dtype == DType::f64) throw TensorError("NonFloatDType");
+  if (!dtypeIsIndex(tokens.dtype)) throw TensorError("NonIntegerDType");
+  vocabularyAxis(logits.dims, tokens.dims);
+  Operation op;
+  op.kind = Kind::custom_call;
+  op.sub = static_cast<uint8_t>(call);
+  op.target = callTarget(call);
+  op.operands = operands;
+  if (call == Call::token_log_prob) {
+    // f32 whatever the logits' type: eight or eleven bits of a log-probability are no use to a loss
+    op.result = Type{DType::f32, tokens.dims};
+  } else {
+    requireSameType(typeOf(operands[2]), Type{DType::f32, tokens.dims});
+    op.result = logits;
+  }
+  return emit(std::move(op));
+}
+
+uint32_t Builder::gatherNamed(uint32_t data, uint32_t indices, const std::string& axis) {
+  ensure(data);
+  const long at = findDim(typeOf(data).dims, axis);
+  if (at < 0) throw TensorError("AxisNotFound");
+  return gather(data, indices, at);
+}
+
+uint32_t Builder::scatterAddNamed(uint32_t base, uint32_t indices, uint32_t updates, const std::string& axis) {
+  ensure(base);
+  ensure(indices);
+  ensure(updates);
+  const long at = findDim(typeOf(base).dims, axis);
+  if (at < 0) throw TensorError("AxisNotFound");
+  // updates may come in any axis order, and without the axes they are the same along
+  return scatterAdd(base, indices, alignTo(updates, replacedAxis(typeOf(base).dims, at, typeOf(indices).dims)), at);
+}
+
+uint32_t Builder::tokenLogProbNamed(uint32_t logits, uint32_t tokens, const std::string& axis) {
+  ensure(logits);
+  ensure(tokens);
+  const long at = findDim(typeOf(logits).dims, axis);
+  if (at < 0) throw TensorError("AxisNotFound");
+  return customCall(Call::token_log_prob, {logits, alignTo(tokens, replacedAxis(typeOf(logits).dims, at, {}))});
 }
 
 uint32_t Builder::alignTo(uint32_t x, const std::vector<Dim>& target) {

@@ -19,6 +19,7 @@ constexpr uint32_t kDTypeCount = 14;
 size_t dtypeSize(DType d);
 const char* dtypeName(DType d);
 bool dtypeIsFloat(DType d);
+bool dtypeIsIndex(DType d);  // the integer types a gather, a scatter_add or a token may be numbered with
 
 // Operation kinds in wire order (src/tensor/wire/format.zig:79-99).
 enum class Kind : uint8_t {
@@ -33,6 +34,14 @@ enum class Unary : uint8_t { neg, abs, exp, log, sqrt, tanh, sin, cos, tan };
 enum class Binary : uint8_t { add, sub, mul, div, max, min, pow };
 enum class Reducer : uint8_t { sum, max, min };
 enum class Compare : uint8_t { lt, le, gt, ge, eq, ne };
+// The custom calls this target knows, by wire target name and version (`customCallOf`); any other is refused.
+enum class Call : uint8_t {
+  token_log_prob,       // (logits, tokens): f32 log-probability of one token per row
+  token_log_prob_grad,  // (logits, tokens, slope f32): its gradient with respect to the logits, times the rows' slopes
+};
+constexpr uint32_t kCallCount = 2;
+const char* callTarget(Call c);
+bool customCallOf(const std::string& target, uint32_t version, Call* call);
 
 struct Dim {
   std::string name;
@@ -57,7 +66,7 @@ struct Operation {
   uint32_t id = 0;
   Type result;
   Kind kind = Kind::parameter;
-  uint8_t sub = 0;                  // Unary / Binary / Reducer / Compare code
+  uint8_t sub = 0;                  // Unary / Binary / Reducer / Compare / Call code
   std::vector<uint32_t> operands;   // value ids, in the reference's field order
   std::vector<int64_t> ints;        // broadcast_dims | permutation | reduce dimensions | lhs_contract
   std::vector<int64_t> rhs_contract, lhs_batch, rhs_batch;  // dot_general only
@@ -93,6 +102,10 @@ Alignment alignment(const std::vector<Dim>& operand, const std::vector<Dim>& tar
 std::vector<int64_t> axisIndices(const std::vector<Dim>& dims, const std::vector<std::string>& names);
 std::vector<Dim> removeAxes(const std::vector<Dim>& dims, const std::vector<int64_t>& axes);
 std::vector<Dim> permuted(const std::vector<Dim>& dims, const std::vector<int64_t>& permutation);
+// `dims` with the dim at `axis` replaced by `by` (the type of a gather)
+std::vector<Dim> replacedAxis(const std::vector<Dim>& dims, int64_t axis, const std::vector<Dim>& by);
+// The one dim of `logits` that `tokens` lacks; the others have to be the same, in the same order.
+size_t vocabularyAxis(const std::vector<Dim>& logits, const std::vector<Dim>& tokens);
 
 struct Contraction {
   std::vector<int64_t> lhs_contract, rhs_contract, lhs_batch, rhs_batch;
@@ -142,6 +155,14 @@ class Builder {
                         const std::vector<int64_t>& rhs_contract,
                         const std::vector<int64_t>& lhs_batch,
                         const std::vector<int64_t>& rhs_batch);
+  // Lookups by number (the wire's `gather` and `scatter_add`).  The axis of `data` is replaced by the
+  // axes of `indices`; a number outside [0, extent) reads zeros and adds nothing.
+  uint32_t gather(uint32_t data, uint32_t indices, int64_t axis);
+  uint32_t scatterAdd(uint32_t base, uint32_t indices, uint32_t updates, int64_t axis);
+  uint32_t customCall(Call call, const std::vector<uint32_t>& operands);
+  uint32_t gatherNamed(uint32_t data, uint32_t indices, const std::string& axis);
+  uint32_t scatterAddNamed(uint32_t base, uint32_t indices, uint32_t updates, const std::string& axis);
+  uint32_t tokenLogProbNamed(uint32_t logits, uint32_t tokens, const std::string& axis);
   uint32_t alignTo(uint32_t x, const std::vector<Dim>& target);
   Program finish(const std::vector<uint32_t>& outputs);
 

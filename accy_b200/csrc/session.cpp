@@ -397,24 +397,29 @@ struct accy_b200_session {
     const bool record_events = time_it && time_launches;
     if (record_events) check(d.cuEventRecord(e.ev_begin, on), "cuEventRecord");
     static const bool graphs_off = std::getenv("ACCY_B200_NO_GRAPHS") != nullptr;
-    const bool replayable = time_it && !graphs_off && e.plan.launches.size() >= 2 && e.graph_recordings < 4;
+    bool replayable = time_it && !graphs_off && e.plan.launches.size() >= 2 && e.graph_recordings < 4;
+    // A stream that the caller is capturing takes the kernels themselves: its own graph replays them, and
+    // neither a recording nor a graph launch may happen in the middle of it.
+    int capturing = 0;
+    if (replayable && d.cuStreamIsCapturing(on, &capturing) == 0 && capturing != 0) replayable = false;
     bool submitted = false;
     if (replayable && e.graph && e.graph_bound == e.bound) {
       submitted = d.cuGraphLaunch(e.graph, on) == 0;
       if (!submitted) e.graph_recordings = 4;  // give up on graphs for this program, launch directly below
-    } else if (replayable && d.cuStreamBeginCapture(on, 2 /* relaxed: other threads' calls do not matter */) == 0) {
+    } else if (replayable && d.cuStreamBeginCapture(stream, 2 /* relaxed: other threads' calls do not matter */) == 0) {
+      // recorded on the session's own stream: the legacy default stream (handle 1) cannot be captured
       if (e.graph) d.cuGraphExecDestroy(e.graph);
       e.graph = nullptr;
       e.graph_recordings += 1;
       CUgraph_t recorded = nullptr;
       try {
-        issueLaunches(e, on);
+        issueLaunches(e, stream);
       } catch (...) {
-        d.cuStreamEndCapture(on, &recorded);
+        d.cuStreamEndCapture(stream, &recorded);
         if (recorded) d.cuGraphDestroy(recorded);
         throw;
       }
-      if (d.cuStreamEndCapture(on, &recorded) == 0 && recorded &&
+      if (d.cuStreamEndCapture(stream, &recorded) == 0 && recorded &&
           d.cuGraphInstantiateWithFlags(&e.graph, recorded, 0) == 0 && d.cuGraphLaunch(e.graph, on) == 0) {
         e.graph_bound = e.bound;
         submitted = true;
@@ -947,6 +952,20 @@ uint32_t accy_b200_builder_mean(accy_b200_builder* b, uint32_t x, const char* co
 uint32_t accy_b200_builder_contract(accy_b200_builder* b, uint32_t lhs, uint32_t rhs, const char* const* axes,
                                     uint32_t axis_count, uint32_t* value) {
   return built(b, value, [&] { return b->builder.contract(lhs, rhs, namesOf(axes, axis_count)); });
+}
+
+uint32_t accy_b200_builder_gather(accy_b200_builder* b, uint32_t data, uint32_t indices, const char* axis, uint32_t* value) {
+  return built(b, value, [&] { return b->builder.gatherNamed(data, indices, axis ? axis : ""); });
+}
+
+uint32_t accy_b200_builder_scatter_add(accy_b200_builder* b, uint32_t base, uint32_t indices, uint32_t updates,
+                                       const char* axis, uint32_t* value) {
+  return built(b, value, [&] { return b->builder.scatterAddNamed(base, indices, updates, axis ? axis : ""); });
+}
+
+uint32_t accy_b200_builder_token_log_prob(accy_b200_builder* b, uint32_t logits, uint32_t tokens, const char* axis,
+                                          uint32_t* value) {
+  return built(b, value, [&] { return b->builder.tokenLogProbNamed(logits, tokens, axis ? axis : ""); });
 }
 
 uint32_t accy_b200_builder_rename(accy_b200_builder* b, uint32_t x, const char* old_name, const char* new_name, uint32_t* value) {

@@ -22,6 +22,15 @@ namespace accy {
 
 namespace {
 
+// Whether a value is zeros everywhere: a zero constant, or one broadcast to its dims.
+bool isZeros(const Program& p, uint32_t id) {
+  while (p.ops[id].kind == Kind::broadcast_in_dim || p.ops[id].kind == Kind::broadcast) id = p.ops[id].operands[0];
+  if (p.ops[id].kind != Kind::constant) return false;
+  for (uint8_t byte : p.ops[id].payload)
+    if (byte) return false;
+  return true;
+}
+
 bool hasAxis(const Type& t, const std::string& axis) { return findDim(t.dims, axis) >= 0; }
 
 std::vector<Dim> resized(const std::vector<Dim>& dims, const std::string& axis, int64_t extent) {
@@ -104,6 +113,29 @@ ShardInfo analyseShardAxis(const Program& p, const std::string& axis) {
           if (lhs.dims[d].name == axis) { info.reason = "the axis is contracted"; return info; }
         break;
       }
+      case Kind::gather:
+        if (p.typeOf(op.operands[0]).dims[op.axis].name == axis) { info.reason = "rows are looked up along the axis"; return info; }
+        break;
+      case Kind::scatter_add: {
+        if (op.result.dims[op.axis].name == axis) { info.reason = "rows are scattered along the axis"; return info; }
+        if (!hasAxis(p.typeOf(op.operands[1]), axis)) break;
+        // each piece adds its own updates: a final sum over the axis, which every piece starts from the
+        // base, so the base has to be zeros
+        if (!is_output[op.id]) { info.reason = "updates along the axis are summed inside the program"; return info; }
+        if (!isZeros(p, op.operands[0])) { info.reason = "the base of a scatter_add over the axis is not zeros"; return info; }
+        if (info.partial_fold > 1) { info.reason = "outputs fold the axis with different reducers"; return info; }
+        info.partial_fold = 1;
+        info.partial_outputs.push_back(op.id);
+        break;
+      }
+      case Kind::custom_call: {
+        const Type& logits = p.typeOf(op.operands[0]);
+        if (logits.dims[vocabularyAxis(logits.dims, p.typeOf(op.operands[1]).dims)].name == axis) {
+          info.reason = "the axis is the vocabulary of a log-probability";
+          return info;
+        }
+        break;
+      }
       case Kind::reshape: {
         const Type& in = p.typeOf(op.operands[0]);
         long in_at = findDim(in.dims, axis);
@@ -182,6 +214,9 @@ Program shardProgram(const Program& p, const std::string& axis, int64_t extent) 
       case Kind::dot_general:
         made = b.dotGeneralOp(op.operands[0], op.operands[1], op.ints, op.rhs_contract, op.lhs_batch, op.rhs_batch);
         break;
+      case Kind::gather: made = b.gather(op.operands[0], op.operands[1], op.axis); break;
+      case Kind::scatter_add: made = b.scatterAdd(op.operands[0], op.operands[1], op.operands[2], op.axis); break;
+      case Kind::custom_call: made = b.customCall(static_cast<Call>(op.sub), op.operands); break;
       default:
         throw PlanError("operation kind not shardable");
     }

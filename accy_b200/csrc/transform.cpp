@@ -60,7 +60,13 @@ uint32_t replayUnchanged(Builder& b, const Operation& op, const std::vector<uint
     case Kind::reduce: return b.reduce(arg(0), arg(1), static_cast<Reducer>(op.sub), op.ints);
     case Kind::dot_general:
       return b.dotGeneralOp(arg(0), arg(1), op.ints, op.rhs_contract, op.lhs_batch, op.rhs_batch);
-    case Kind::custom_call: throw TensorError("CustomCallRequiresJvpContract");
+    case Kind::gather: return b.gather(arg(0), arg(1), op.axis);
+    case Kind::scatter_add: return b.scatterAdd(arg(0), arg(1), arg(2), op.axis);
+    case Kind::custom_call: {
+      std::vector<uint32_t> operands;
+      for (uint32_t id : op.operands) operands.push_back(now[id]);
+      return b.customCall(static_cast<Call>(op.sub), operands);
+    }
     case Kind::scan:
     case Kind::projection: throw TensorError("ScanLinearizationUnsupported");
     default: throw TensorError("OperationUnsupported");
@@ -149,6 +155,22 @@ class Reverse {
       }
       case Kind::reduce: return pullReduce(op, g);
       case Kind::dot_general: return pullDot(op, g);
+      case Kind::gather: {
+        // the rows' cotangents go back to the rows they were read from, on top of what has arrived there already
+        const uint32_t xi = op.operands[0];
+        if (!dtypeIsFloat(src_.typeOf(xi).dtype)) throw TensorError("UnsupportedDerivative");
+        ct_[xi] = b_.scatterAdd(cotangent(xi), now_[op.operands[1]], g, op.axis);
+        return;
+      }
+      case Kind::scatter_add:
+        give(op.operands[0], g);
+        if (wants(op.operands[2])) give(op.operands[2], b_.gather(g, now_[op.operands[1]], op.axis));
+        return;
+      case Kind::custom_call: {
+        if (static_cast<Call>(op.sub) != Call::token_log_prob) throw TensorError("UnsupportedDerivative");
+        const uint32_t xi = op.operands[0];
+        return give(xi, b_.customCall(Call::token_log_prob_grad, {now_[xi], now_[op.operands[1]], g}));
+      }
       default: return;  // parameter, constant, iota, compare: nothing upstream
     }
   }
@@ -539,6 +561,28 @@ class Forward {
         tan_[op.id] = left && right ? bin(Binary::add, *left, *right) : (left ? *left : right.value());
         return;
       }
+      case Kind::gather:
+        if (t(0)) tan_[op.id] = b_.gather(*t(0), x(1), op.axis);
+        return;
+      case Kind::scatter_add: {
+        const Opt tb = t(0), tu = t(2);
+        if (tu) tan_[op.id] = b_.scatterAdd(tb ? *tb : zerosLike(op.operands[0]), x(1), *tu, op.axis);
+        else tan_[op.id] = tb;   // no tangent arrives with the updates
+        return;
+      }
+      case Kind::custom_call: {
+        // d log p = sum over the vocabulary of (d log p / d logits) * d logits; the sum is typed like
+        // the logits, the result f32, and no operation converts between them
+        for (size_t i = 1; i < op.operands.size(); ++i)
+          if (t(i)) throw TensorError("UnsupportedDerivative");
+        if (!t(0)) return;
+        const Type& ty = src_.typeOf(op.operands[0]);
+        if (static_cast<Call>(op.sub) != Call::token_log_prob || ty.dtype != DType::f32) throw TensorError("UnsupportedDerivative");
+        const int64_t axis = static_cast<int64_t>(vocabularyAxis(ty.dims, src_.typeOf(op.operands[1]).dims));
+        const uint32_t slope = b_.customCall(Call::token_log_prob_grad, {x(0), x(1), filled(b_, op.result, 1.0)});
+        tan_[op.id] = b_.reduce(bin(Binary::mul, slope, *t(0)), b_.fullFloat(Type{ty.dtype, {}}, 0.0), Reducer::sum, {axis});
+        return;
+      }
       default: return;  // constant, iota, compare: no tangent
     }
   }
@@ -669,9 +713,58 @@ class Vmap {
         return {b_.reduce(arg(0).id, arg(1).id, static_cast<Reducer>(op.sub), shifted(op.ints)), true};
       }
       case Kind::dot_general: return dot(op, arg(0), arg(1));
-      case Kind::custom_call: throw TensorError("CustomCallRequiresBatchContract");
+      case Kind::gather: {
+        const Batched &data = arg(0), &indices = arg(1);
+        if (!indices.mapped) return {b_.gather(data.id, indices.id, op.axis + 1), true};
+        // the new axis arrives with the indices: it lands where the looked-up axis was
+        if (!data.mapped) return {frontAxis(b_.gather(data.id, indices.id, op.axis), static_cast<size_t>(op.axis)), true};
+        const Type ty = b_.typeOf(data.id);
+        return {b_.gather(b_.reshapeTo(data.id, joined(ty, op.axis)), rowsOf(indices.id, ty, op.axis), 0), true};
+      }
+      case Kind::scatter_add: {
+        const uint32_t base = lifted(arg(0)), updates = lifted(arg(2));
+        if (!arg(1).mapped) return {b_.scatterAdd(base, arg(1).id, updates, op.axis + 1), true};
+        const Type ty = b_.typeOf(base);
+        const uint32_t rows = b_.reshapeTo(base, joined(ty, op.axis));
+        return {b_.reshapeTo(b_.scatterAdd(rows, rowsOf(arg(1).id, ty, op.axis), updates, 0), ty.dims), true};
+      }
+      case Kind::custom_call: {
+        std::vector<uint32_t> operands;
+        for (uint32_t id : op.operands) operands.push_back(lifted(now[id]));
+        return {b_.customCall(static_cast<Call>(op.sub), operands), true};
+      }
       default: throw TensorError("OperationUnsupported");
     }
+  }
+
+  // Both the looked-up value and the numbers carry the new axis: instance i's rows are rows
+  // [i * extent, (i + 1) * extent) of the two axes read as one, and its numbers move there.
+  static std::vector<Dim> joined(const Type& ty, int64_t axis) {
+    if (axis != 0) throw TensorError("UnsupportedBatching");
+    std::vector<Dim> dims(ty.dims.begin() + 1, ty.dims.end());
+    dims[0] = Dim{"#rows", ty.dims[0].extent * ty.dims[1].extent};
+    return dims;
+  }
+  uint32_t rowsOf(uint32_t indices, const Type& ty, int64_t axis) {
+    const Type it = b_.typeOf(indices);
+    const int64_t extent = ty.dims[1].extent, rows = joined(ty, axis)[0].extent;
+    // every row's number, and for an unsigned type one more for "none of them", has to fit the type
+    const bool is_signed = it.dtype <= DType::i64;
+    const size_t bits = 8 * dtypeSize(it.dtype) - (is_signed ? 1 : 0);
+    if (bits < 63 && rows + (is_signed ? 0 : 1) > (int64_t{1} << bits)) throw TensorError("UnsupportedBatching");
+    auto number = [&](int64_t v) {
+      std::vector<uint8_t> payload(dtypeSize(it.dtype));
+      for (size_t i = 0; i < payload.size(); ++i) payload[i] = static_cast<uint8_t>(static_cast<uint64_t>(v) >> (8 * i));
+      const uint32_t scalar = b_.constantBytes(Type{it.dtype, {}}, payload.data(), payload.size());
+      return b_.broadcastTo(scalar, it.dims, {});
+    };
+    // numbers outside their own instance's rows stay outside all of them.  Compared with the last row: the
+    // extent itself may be one more than the type holds.
+    if (extent == 0) return indices;
+    const uint32_t low = b_.compare(Compare::ge, indices, number(0)), high = b_.compare(Compare::le, indices, number(extent - 1));
+    const uint32_t moved = b_.binary(Binary::add, indices, b_.binary(Binary::mul, b_.iotaTyped(it, 0), number(extent)));
+    const uint32_t outside = is_signed ? number(-1) : number(rows);
+    return b_.select(low, b_.select(high, moved, outside), outside);
   }
 
   Batched parameter(const Operation& op) {

@@ -259,13 +259,20 @@ Program decodeProgram(const uint8_t* bytes, size_t len) {
         break;
       }
       case Kind::custom_call: {
-        (void)r.typed();
-        (void)r.str();
-        (void)r.u32();
+        const Type declared = r.typed();
+        const std::string target = r.str();
+        const uint32_t version = r.u32();
         uint32_t cnt = r.count(4);
         if (cnt > kMaxCustomCallOperands) throw WireError("TooManyOperands");
-        for (uint32_t i = 0; i < cnt; ++i) (void)r.id(limit);
-        throw WireError("CustomCallUnsupported");
+        std::vector<uint32_t> operands(cnt);
+        for (uint32_t& id : operands) id = r.id(limit);
+        Call call;
+        if (!customCallOf(target, version, &call)) throw WireError("CustomCallUnsupported");
+        made = builder.customCall(call, operands);
+        // the declared type is not trusted: it has to be the one the call has
+        const Type& derived = builder.typeOf(made);
+        if (declared.dtype != derived.dtype || !sameDims(declared.dims, derived.dims)) throw WireError("InvalidProgram");
+        break;
       }
       case Kind::broadcast: {
         std::vector<Dim> dims = r.dims();
@@ -322,9 +329,17 @@ Program decodeProgram(const uint8_t* bytes, size_t len) {
         made = builder.dotGeneralOp(lhs, rhs, lc, rc, lb, rb);
         break;
       }
+      case Kind::gather: {
+        uint32_t data = r.id(limit), indices = r.id(limit);
+        made = builder.gather(data, indices, r.i64());
+        break;
+      }
+      case Kind::scatter_add: {
+        uint32_t base = r.id(limit), indices = r.id(limit), updates = r.id(limit);
+        made = builder.scatterAdd(base, indices, updates, r.i64());
+        break;
+      }
       case Kind::projection:
-      case Kind::gather:
-      case Kind::scatter_add:
       case Kind::sparse_cross_entropy:
         throw WireError("OperationUnsupported");
       case Kind::scan:

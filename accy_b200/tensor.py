@@ -232,6 +232,25 @@ class Value:
         names, count = _axes(axes)
         return self.builder._emit(lib.accy_b200_builder_contract, self.id, self.builder._check(rhs), names, count)
 
+    def gather(self, indices, axis):
+        """This value with `axis` replaced by the axes of the integer value `indices`: the rows they number.
+        A number outside [0, extent) reads zeros."""
+        b = self.builder
+        return b._emit(lib.accy_b200_builder_gather, self.id, b._check(indices), axis.encode())
+
+    def scatter_add(self, indices, updates, axis):
+        """This value plus, at every row of `axis`, the `updates` that `indices` numbers with it, summed in the
+        order of the indices; a number outside [0, extent) adds nothing.  `updates` has the axes of
+        `gather(indices, axis)`, or lacks those it is the same along."""
+        b = self.builder
+        return b._emit(lib.accy_b200_builder_scatter_add, self.id, b._check(indices), b._check(updates), axis.encode())
+
+    def token_log_prob(self, tokens, axis):
+        """f32 log-probability of `tokens` (this value without `axis`, integers) under the softmax of this value
+        along `axis`; 0, with a zero gradient, for a token outside [0, extent)."""
+        b = self.builder
+        return b._emit(lib.accy_b200_builder_token_log_prob, self.id, b._check(tokens), axis.encode())
+
     def rename(self, old_name, new_name):
         return self.builder._emit(lib.accy_b200_builder_rename, self.id, old_name.encode(), new_name.encode())
 

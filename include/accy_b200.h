@@ -108,7 +108,9 @@ uint32_t accy_b200_session_invoke(accy_b200_session* session, uint64_t handle,
                                   const size_t* output_sizes, uint32_t output_count);
 /* The same launch on buffers already in device memory (the vtable's launch on caller-allocated
  * buffers, contract.zig:2048-2085): no copies, asynchronous on `stream` (a CUstream, or NULL for
- * the session's own stream).  Pointers must be 256-byte aligned.  Launches of one handle must not
+ * the session's own stream; the legacy default stream has the handle 1).  A stream the caller is
+ * capturing takes the program's kernels into the caller's graph, which may be replayed while the
+ * program is held.  Pointers must be 256-byte aligned.  Launches of one handle must not
  * overlap on the device (put them on one stream or order them with events): they share the
  * program's temporaries, scratch and work counters. */
 uint32_t accy_b200_session_invoke_device(accy_b200_session* session, uint64_t handle,
@@ -176,6 +178,24 @@ uint32_t accy_b200_builder_mean(accy_b200_builder* b, uint32_t x, const char* co
                                 uint32_t* value);
 uint32_t accy_b200_builder_contract(accy_b200_builder* b, uint32_t lhs, uint32_t rhs, const char* const* axes,
                                     uint32_t axis_count, uint32_t* value);
+/* Lookups by number.  gather: the named axis of `data` is replaced by the axes of `indices` (any integer
+ * type but i1): out[.., i.., ..] = data[.., indices[i..], ..].  scatter_add: `base` plus, at every row
+ * of the axis, the updates numbered with it, summed in f32 (f64 for f64) in the order of the indices,
+ * the same on every run; `updates` has the type of gather(base, indices) and may lack axes it is the same along.
+ * A number outside [0, extent) reads zeros and adds nothing.  These are the wire's `gather` (data,
+ * indices, axis) and `scatter_add` (base, indices, updates, axis) operations. */
+uint32_t accy_b200_builder_gather(accy_b200_builder* b, uint32_t data, uint32_t indices, const char* axis,
+                                  uint32_t* value);
+uint32_t accy_b200_builder_scatter_add(accy_b200_builder* b, uint32_t base, uint32_t indices, uint32_t updates,
+                                       const char* axis, uint32_t* value);
+/* The log-probability of one token per row: f32 out[r..] = x[r.., t] - log(sum_v exp(x[r.., v])) with
+ * t = tokens[r..], x = `logits` (f32, bf16 or f16) and v along the named axis, which `tokens` (any
+ * integer type but i1) lacks; 0, with a zero gradient, where t is outside [0, extent).  On the wire this
+ * is the custom call "accy_b200.token_log_prob" version 1; wire_grad records its gradient as
+ * "accy_b200.token_log_prob_grad" (logits, tokens, slope f32[r..]): (1[v = t] - softmax(x)[v]) * slope,
+ * and zeros for a row whose slope is zero, whatever its logits are. */
+uint32_t accy_b200_builder_token_log_prob(accy_b200_builder* b, uint32_t logits, uint32_t tokens, const char* axis,
+                                          uint32_t* value);
 uint32_t accy_b200_builder_rename(accy_b200_builder* b, uint32_t x, const char* old_name, const char* new_name,
                                   uint32_t* value);
 uint32_t accy_b200_builder_split(accy_b200_builder* b, uint32_t x, const char* axis, const char* const* names,

@@ -219,6 +219,31 @@ def decode(data):
             if init.dims:
                 raise OracleError("ReduceInitNotScalar")
             op.dtype, op.dims = src.dtype, _remove_axes(src.dims, op.ints)
+        elif k in ("gather", "scatter_add"):
+            # data / base, indices[, updates], axis: the axis is replaced by the axes of the indices
+            op.operands = [ref() for _ in range(2 if k == "gather" else 3)]
+            op.axis = r.i64()
+            src, idx = ops[op.operands[0]], ops[op.operands[1]]
+            if not 0 <= op.axis < len(src.dims):
+                raise OracleError("AxisOutOfRange")
+            rows = src.dims[:op.axis] + idx.dims + src.dims[op.axis + 1:]
+            if k == "scatter_add" and (ops[op.operands[2]].dims != rows or ops[op.operands[2]].dtype != src.dtype):
+                raise OracleError("ShapeMismatch")
+            op.dtype, op.dims = src.dtype, list(rows if k == "gather" else src.dims)
+        elif k == "custom_call":
+            declared = r.typed()
+            op.sub, version = r.blob().decode(), r.u32()
+            op.operands = [ref() for _ in range(r.u32())]
+            if op.sub not in ("accy_b200.token_log_prob", "accy_b200.token_log_prob_grad") or version != 1:
+                raise OracleError("CustomCallUnsupported")
+            x, tok = ops[op.operands[0]], ops[op.operands[1]]
+            lacking = [i for i, d in enumerate(x.dims) if d not in tok.dims]
+            if len(lacking) != 1 or _remove_axes(x.dims, lacking) != tok.dims:
+                raise OracleError("ShapeMismatch")
+            op.axis = lacking[0]
+            op.dtype, op.dims = ("f32", list(tok.dims)) if op.sub.endswith("prob") else (x.dtype, list(x.dims))
+            if (op.dtype, op.dims) != (declared[0], list(declared[1])):
+                raise OracleError("InvalidProgram")
         elif k == "dot_general":
             op.operands = [ref(), ref()]
             op.lists = [r.ints(), r.ints(), r.ints(), r.ints()]
@@ -255,6 +280,40 @@ def f32_to_bf16(a, truncate=False):
 
 def _shape(dims):
     return tuple(e for _, e in dims)
+
+
+def _lookup(x, idx, axis):
+    """x with `axis` replaced by the axes of idx; zeros where a number is outside the axis."""
+    rows = np.moveaxis(x, axis, 0)
+    known = (idx >= 0) & (idx < len(rows))
+    picked = rows[np.where(known, idx, 0).astype(np.int64)] if len(rows) else np.zeros(idx.shape + rows.shape[1:], x.dtype)
+    picked = np.where(known.reshape(known.shape + (1,) * (rows.ndim - 1)), picked, 0).astype(x.dtype)
+    # the index axes go where the looked-up axis was
+    return np.ascontiguousarray(np.moveaxis(picked, list(range(idx.ndim)), list(range(axis, axis + idx.ndim))))
+
+
+def _scatter_add(base, idx, updates, axis):
+    out = np.moveaxis(base.copy(), axis, 0)
+    rows = np.moveaxis(updates, list(range(axis, axis + idx.ndim)), list(range(idx.ndim))).reshape((idx.size,) + out.shape[1:])
+    for i, v in enumerate(idx.reshape(-1)):
+        if 0 <= v < len(out):
+            out[int(v)] += rows[i]
+    return np.ascontiguousarray(np.moveaxis(out, 0, axis))
+
+
+def _token_log_prob(x, tok, axis):
+    """(log-probability of each token, probabilities, one-hot of the tokens): zero rows for a token outside."""
+    known = (tok >= 0) & (tok < x.shape[axis])
+    at = np.expand_dims(np.where(known, tok, 0).astype(np.int64), axis)
+    hot = np.zeros_like(x)
+    with np.errstate(all="ignore"):
+        shifted = x - x.max(axis, keepdims=True)
+        e = np.exp(shifted)
+        total = e.sum(axis, keepdims=True)
+        log_prob = np.squeeze(np.take_along_axis(shifted, at, axis) - np.log(total), axis)
+        p = e / total
+    np.put_along_axis(hot, at, np.expand_dims(known, axis).astype(x.dtype), axis)
+    return np.where(known, log_prob, 0).astype(x.dtype), p, hot
 
 
 class Evaluator:
@@ -405,6 +464,22 @@ class Evaluator:
                 vals[op.id] = self._round(op.dtype, self._reduce(op.sub, init, vals[op.operands[0]], op.ints))
             elif k == "dot_general":
                 vals[op.id] = self._round(op.dtype, self._dot(vals[op.operands[0]], vals[op.operands[1]], op.lists))
+            elif k == "gather":
+                x, idx = vals[op.operands[0]], vals[op.operands[1]]
+                vals[op.id] = _lookup(x, idx, op.axis)
+            elif k == "scatter_add":
+                base, idx, up = (vals[i] for i in op.operands)
+                vals[op.id] = self._round(op.dtype, _scatter_add(base, idx, up, op.axis))
+            elif k == "custom_call":
+                x, tok = vals[op.operands[0]], vals[op.operands[1]]
+                log_prob, p, hot = _token_log_prob(x, tok, op.axis)
+                if op.sub.endswith("prob"):
+                    vals[op.id] = log_prob
+                else:
+                    g = np.expand_dims(vals[op.operands[2]], op.axis)
+                    with np.errstate(all="ignore"):
+                        grad = np.where((g == 0) | (hot.sum(op.axis, keepdims=True) == 0), 0, (hot - p) * g).astype(x.dtype)
+                    vals[op.id] = self._round(op.dtype, grad)
             else:
                 raise OracleError("unsupported kind " + k)
         result = []
