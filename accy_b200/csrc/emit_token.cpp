@@ -502,30 +502,20 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
 // ---------------------------------------------------------------------------------------------
 namespace {
 
-// One row of logits per TPR threads (CL CTAs of a cluster share a long row).  A thread loads its part of
-// the row once, folds its maximum m and its sum of 2^((x - m) log2 e), and the row's (m, sum) pairs are
-// combined through shuffles, shared memory and, in a cluster, distributed shared memory:
+// The arithmetic.  With c = fl(m log2 e) for a reference m near the row's maximum,
 //
-//   log p = (x[token] - m) - log(sum)         d log p / d x[v] = 1[v = token] - 2^((x[v] - m) log2 e) / sum
+//   e[v] = 2^(x[v] log2 e - c)    log p = ln 2 (x[token] log2 e - c) - ln(sum e)    p[v] = e[v] / sum e
 //
-// The gradient is written from the registers that hold the row, so logits are read once and the gradient
-// written once; the slope of each row (what the recorded program does to its log-probability on the
-// way to the loss) is evaluated in between.  Rows need not be aligned: a row is covered by aligned
-// 16-byte vectors, and the elements of the first and last one that belong to its neighbours are left out.
-const char* kTokenTemplate = R"CUDA(
+// one fused step and one ex2.approx per element.  c is the same for every element that is summed with it
+// or divided by the sum, so its rounding cancels, and the fused step rounds at the size of its result: rows whose
+// logits are all far from zero lose nothing.  References are combined as 2^(c1 - c2), for the same
+// reason.  A reference of 1e38 or more would overflow c: such rows (logits at the type's lowest value)
+// subtract first.  A thread moves its reference only when a logit exceeds it by more than 40: e^40 times
+// any number of terms is far from the end of f32, and the sums then rarely need rescaling.
+const char* kTokenCommon = R"CUDA(
 #define L2E 1.4426950408889634f
-__device__ __forceinline__ float2 peer_pair(const float2* p, unsigned int cta) {
-  const unsigned int a = (unsigned int)__cvta_generic_to_shared(p);
-  unsigned int b;
-  float2 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(a), "r"(cta));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(b) : "memory");
-  return v;
-}
-__device__ __forceinline__ float finite_or_zero_ref(float m) { return m == __uint_as_float(0xff800000u) ? 0.0f : m; }
-// the sum `s` relative to the maximum m, seen relative to `ref`
-__device__ __forceinline__ float rescaled(float s, float m, float ref) { return s * ex2_ftz((m - ref) * L2E); }
-
+#define LN2 0.6931471805599453f
+#define NEG_INF __uint_as_float(0xff800000u)
 #if IN_BITS == 32
 __device__ __forceinline__ float value_of(XT x) { return x; }
 #define NEG_INF_WORD 0xff800000u
@@ -537,7 +527,7 @@ __device__ __forceinline__ float value_of(XT x) { return f16_to_f32(x); }
 #define NEG_INF_WORD 0xfc00fc00u
 #endif
 
-struct Raw { unsigned int w[4]; };
+struct Raw { unsigned int w[4]; };   // 16 bytes of a row
 
 __device__ __forceinline__ void unpack(const Raw& v, float (&f)[E]) {
 #pragma unroll
@@ -548,8 +538,7 @@ __device__ __forceinline__ void unpack(const Raw& v, float (&f)[E]) {
     f[2 * i] = __uint_as_float(v.w[i] << 16);
     f[2 * i + 1] = __uint_as_float(v.w[i] & 0xffff0000u);
 #else
-    f[2 * i] = f16_to_f32((unsigned short)(v.w[i] & 0xffffu));
-    f[2 * i + 1] = f16_to_f32((unsigned short)(v.w[i] >> 16));
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}" : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "r"(v.w[i]));
 #endif
   }
 }
@@ -563,20 +552,188 @@ __device__ __forceinline__ unsigned int packed_max(unsigned int a, unsigned int 
   unsigned int r; asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r;
 #endif
 }
+__device__ __forceinline__ float largest(unsigned int packed) {
+#if IN_BITS == 32
+  return __uint_as_float(packed);
+#else
+  return fmaxf(value_of((XT)(packed & 0xffffu)), value_of((XT)(packed >> 16)));
+#endif
+}
+// whether c would overflow (f16 logits cannot get there; an infinite one gives NaN either way)
+__device__ __forceinline__ bool huge_ref(float m) {
+#if IN_BITS == 32 || IN_BF16
+  return fabsf(m) >= 1e38f && m != NEG_INF;
+#else
+  return false;
+#endif
+}
+// what to add to x log2 e: -c; nothing for a row that has no finite element yet, or that subtracts first
+__device__ __forceinline__ float minus_c(float m) { return m == NEG_INF || huge_ref(m) ? 0.0f : -(m * L2E); }
+// a sum relative to `from` seen relative to `to` >= from (an empty sum has from = -inf)
+__device__ __forceinline__ float moved(float s, float from, float to) {
+  if (to == NEG_INF) return s;
+  return s * ex2_ftz(huge_ref(to) ? (from - to) * L2E : from * L2E + minus_c(to));
+}
+// 2^(x log2 e - c) of a vector.  HUGE, the rare case, is a template argument and not a condition here:
+// the compiler would execute it under a predicate for every element.
+template <bool HUGE> __device__ __forceinline__ void exps(const Raw& v, float m, float minus, float (&f)[E]) {
+  unpack(v, f);
+  if (HUGE) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = f[e] - m;
+  }
+  const unsigned long long scale = pk2(L2E, L2E), add = pk2(minus, minus);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    float a, b;
+    upk2(fma2(pk2(f[e], f[e + 1]), scale, add), a, b);
+    f[e] = ex2_ftz(a);
+    f[e + 1] = ex2_ftz(b);
+  }
+}
+// a thread's share of a row's sum
+struct Sum {
+  float m, s, limit;
+  __device__ __forceinline__ Sum() : m(NEG_INF), s(0.0f), limit(NEG_INF) {}
+  template <int N> __device__ __forceinline__ void fold(const Raw (&raw)[N]) {
+    unsigned int top = raw[0].w[0];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) top = packed_max(top, raw[i].w[q]);
+    const float t = largest(top);
+    if (t > limit) {
+      s = moved(s, m, t);
+      m = t;
+      limit = t + 40.0f;
+    }
+    if (huge_ref(m)) add<true>(raw);
+    else add<false>(raw);
+  }
+  template <bool HUGE, int N> __device__ __forceinline__ void add(const Raw (&raw)[N]) {
+    const float minus = minus_c(m);
+    unsigned long long acc = pk2(s, 0.0f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float f[E];
+      exps<HUGE>(raw[i], m, minus, f);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) acc = add2(acc, pk2(f[e], f[e + 1]));
+    }
+    float lo, hi;
+    upk2(acc, lo, hi);
+    s = lo + hi;
+  }
+  // the sum over W neighbouring lanes, in every one of them
+  template <int W> __device__ __forceinline__ void across_lanes() {
+    float top = m;
+    if (W == 32) {
+      asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(m));
+    } else {
+#pragma unroll
+      for (int off = W / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off, W));
+    }
+    s = moved(s, m, top);
+    m = top;
+#pragma unroll
+    for (int off = W / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off, W);
+  }
+};
+__device__ __forceinline__ float log_prob_at(float x, float m, float total) {
+  const float d = huge_ref(m) ? x - m : __fmaf_rn(x, L2E, minus_c(m)) * LN2;
+  return d - logf(total);
+}
+
+#if GRADIENT
+__device__ __forceinline__ void store_vector(GT* p, const float (&f)[E]) {
+#if OUT_16
+  unsigned int w[E / 2];
+#pragma unroll
+  for (int e = 0; e < E; e += 2) asm("cvt.rn." OUT_16_NAME "x2.f32 %0, %1, %2;" : "=r"(w[e / 2]) : "f"(f[e + 1]), "f"(f[e]));
+#if IN_BITS == 32
+  WRITE(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
+#else
+  WRITE(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+#endif
+#else
+#pragma unroll
+  for (int e = 0; e < E; e += 4) WRITE(reinterpret_cast<float4*>(p + e), make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]));
+#endif
+}
+// What a row's gradient is made of: k = -slope / sum, the slope, and the vector with the token's element.
+struct Slope {
+  float m, minus, k, g, x;
+  long long at;
+  int vector;
+  __device__ __forceinline__ Slope(float m_, float total, float slope, bool known, long long tok, float x_, int lead)
+      : m(m_), minus(minus_c(m_)), g(known ? slope : 0.0f), x(x_), at(tok), vector(known ? (int)((tok + lead) / E) : -1) {
+    k = -g / total;
+  }
+  // rows that take the slow way: those the loss does not depend on are zero whatever their logits hold
+  __device__ __forceinline__ bool special() const { return g == 0.0f || huge_ref(m); }
+  template <bool SPECIAL> __device__ __forceinline__ void of(const Raw& v, float (&f)[E]) const {
+    if (SPECIAL && g == 0.0f) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = 0.0f;
+      return;
+    }
+    if (SPECIAL && huge_ref(m)) exps<true>(v, m, minus, f);
+    else exps<false>(v, m, minus, f);
+    const unsigned long long kk = pk2(k, k);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) upk2(mul2(pk2(f[e], f[e + 1]), kk), f[e], f[e + 1]);
+  }
+  // by the thread that wrote the vector with the token's element, after it: that element again
+  __device__ __forceinline__ void token(GT* grow, int j) const {
+    if (j != vector || g == 0.0f) return;
+    const float e = ex2_ftz(huge_ref(m) ? (x - m) * L2E : __fmaf_rn(x, L2E, minus));
+    grow[at] = STORE((e * k + g));
+  }
+};
+// the elements of an edge vector that belong to the row
+__device__ __forceinline__ void store_edge(GT* grow, int first, const float (&f)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (first + e >= 0 && first + e < VOCAB) grow[first + e] = STORE(f[e]);
+}
+#endif
+)CUDA";
+
+// One row of logits per TPR threads (PARTS CTAs of a cluster share a long row while there are few rows).  A
+// thread holds its part of the row in registers (longer rows in chunks), and the row's sums are combined
+// through shuffles, shared memory and, in a cluster, distributed shared memory.  The gradient is written
+// from the registers that hold the row, so logits are read once and the gradient written once; the slope of
+// each row (what the recorded program does to its log-probability on the way to the loss) is evaluated in
+// between.  Rows need not be aligned: a row is covered by aligned 16-byte vectors, and the elements of the first
+// and last one that belong to its neighbours are left out.
+const char* kTokenTemplate = R"CUDA(
+__device__ __forceinline__ float2 peer_pair(const float2* p, unsigned int cta) {
+  const unsigned int a = (unsigned int)__cvta_generic_to_shared(p);
+  unsigned int b;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(a), "r"(cta));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(b) : "memory");
+  return v;
+}
+__device__ __forceinline__ Raw load_inner(const XT* __restrict__ at) {
+  Raw v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "l"(at));
+  return v;
+}
 // vector j of a row whose first element is element `lead` of its first aligned vector; elements outside
 // the row read as -inf
-__device__ __forceinline__ Raw load_vector(const XT* __restrict__ row, int lead, int j) {
+__device__ __forceinline__ Raw load_vector(const XT* __restrict__ row, int lead, int vectors, int j) {
   Raw v;
   const int first = j * E - lead;
-  if (first >= 0 && first + E <= VOCAB) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "l"(row + first));
+  if (j < vectors && first >= 0 && first + E <= VOCAB) {
+    v = load_inner(row + first);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v.w[i] = NEG_INF_WORD;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (first + e < 0 || first + e >= VOCAB) continue;
+      if (j >= vectors || first + e < 0 || first + e >= VOCAB) continue;
 #if IN_BITS == 32
       v.w[e] = __float_as_uint(row[first + e]);
 #else
@@ -586,6 +743,21 @@ __device__ __forceinline__ Raw load_vector(const XT* __restrict__ row, int lead,
     }
   }
   return v;
+}
+
+// whether this thread's vectors of the chunk that starts at vector j1 lie in the row
+__device__ __forceinline__ bool inner_chunk(int j1, int lead) {
+  return j1 * E - lead >= 0 && (j1 + (VPT - 1) * TPR + 1) * E - lead <= VOCAB;
+}
+__device__ __forceinline__ void load_chunk(const XT* mine, const XT* row, int lead, int vectors, int j0, int ck, Raw (&raw)[VPT]) {
+  const int j1 = j0 + ck * (VPT * TPR);
+  if (inner_chunk(j1, lead)) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) raw[i] = load_inner(mine + (ck * VPT + i) * (TPR * E));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) raw[i] = load_vector(row, lead, vectors, j1 + i * TPR);
+  }
 }
 
 extern "C" __global__ void CLUSTER __launch_bounds__(THREADS, MIN_BLOCKS)
@@ -602,162 +774,84 @@ KERNEL(const XT* __restrict__ X, const TT* __restrict__ T, float* __restrict__ l
   const int lead = (int)(((unsigned long long)row & 15ull) / sizeof(XT));
   const int vectors = (lead + VOCAB + E - 1) / E;
   const int j0 = part * (CHUNKS * TPR * VPT) + t;
-  const float xt = known ? value_of(row[tok]) : 0.0f;
+  const XT* mine = row + ((long long)j0 * E - lead);   // this thread's first vector
+  float xt = 0.0f;
   Raw raw[VPT];
 #if STATS_IN
+  if (known) xt = value_of(row[tok]);
   const float2 kept = stats[r];
-  const float ref = kept.x, total = kept.y;
+  const float m = kept.x, total = kept.y;
 #else
-  float m = __uint_as_float(0xff800000u), s = 0.0f;
+  Sum sum;
   for (int ck = 0; ck < CHUNKS; ++ck) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = j0 + (ck * VPT + i) * TPR;
-      if (j < vectors) raw[i] = load_vector(row, lead, j);
-      else {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) raw[i].w[w] = NEG_INF_WORD;
-      }
-    }
-    unsigned int top = NEG_INF_WORD;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) top = packed_max(top, raw[i].w[w]);
-#if IN_BITS == 32
-    const float m2 = fmaxf(m, __uint_as_float(top));
-#else
-    const float m2 = fmaxf(m, fmaxf(value_of((XT)(top & 0xffffu)), value_of((XT)(top >> 16))));
-#endif
-    const float ref2 = finite_or_zero_ref(m2);
-    if (CHUNKS > 1) s = rescaled(s, m, ref2);
-    m = m2;
-    unsigned long long acc = pk2(s, 0.0f);
-    const unsigned long long minus = pk2(-ref2, -ref2), scale = pk2(L2E, L2E);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      float f[E];
-      unpack(raw[i], f);
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        float a, b;
-        upk2(mul2(add2(pk2(f[e], f[e + 1]), minus), scale), a, b);
-        acc = add2(acc, pk2(ex2_ftz(a), ex2_ftz(b)));
-      }
-    }
-    float lo, hi;
-    upk2(acc, lo, hi);
-    s = lo + hi;
+    load_chunk(mine, row, lead, vectors, j0, ck, raw);
+    // behind the first loads: its address has to wait for the token
+    if (ck == 0 && known) xt = value_of(row[tok]);
+    sum.fold(raw);
   }
   // the row's threads: lanes, then warps, then CTAs
-  constexpr int W = TPR < 32 ? TPR : 32;
-  {
-    float top = m;
-#pragma unroll
-    for (int off = W / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off, W));
-    const float ref2 = finite_or_zero_ref(top);
-    s = rescaled(s, m, ref2);
-    m = top;
-#pragma unroll
-    for (int off = W / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off, W);
-  }
+  sum.across_lanes<(TPR < 32 ? TPR : 32)>();
 #if TPR > 32
   __shared__ float2 cells[RPC * (TPR / 32)];
-  if ((t & 31) == 0) cells[sub * (TPR / 32) + (t >> 5)] = make_float2(m, s);
+  if ((t & 31) == 0) cells[sub * (TPR / 32) + (t >> 5)] = make_float2(sum.m, sum.s);
   __syncthreads();
   {
-    float top = __uint_as_float(0xff800000u);
-#pragma unroll
-    for (int w = 0; w < TPR / 32; ++w) top = fmaxf(top, cells[sub * (TPR / 32) + w].x);
-    const float ref2 = finite_or_zero_ref(top);
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < TPR / 32; ++w) {
-      const float2 c = cells[sub * (TPR / 32) + w];
-      sum += rescaled(c.y, c.x, ref2);
-    }
-    m = top;
-    s = sum;
+    const float2 cell = cells[sub * (TPR / 32) + (t & 31) % (TPR / 32)];
+    sum.m = cell.x;
+    sum.s = cell.y;
+    sum.across_lanes<TPR / 32>();
   }
 #endif
 #if CLUSTERED
-  __shared__ float2 mine;
-  if (threadIdx.x == 0) mine = make_float2(m, s);
+  __shared__ float2 whole;
+  if (threadIdx.x == 0) whole = make_float2(sum.m, sum.s);
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
   {
-    float2 c[PARTS];
-    float top = __uint_as_float(0xff800000u);
-#pragma unroll
-    for (int q = 0; q < PARTS; ++q) {
-      c[q] = peer_pair(&mine, q);
-      top = fmaxf(top, c[q].x);
-    }
-    const float ref2 = finite_or_zero_ref(top);
-    float sum = 0.0f;
-#pragma unroll
-    for (int q = 0; q < PARTS; ++q) sum += rescaled(c[q].y, c[q].x, ref2);
-    m = top;
-    s = sum;
+    const float2 theirs = peer_pair(&whole, (threadIdx.x & 31) % PARTS);
+    sum.m = theirs.x;
+    sum.s = theirs.y;
+    sum.across_lanes<PARTS>();
   }
   // nobody leaves while another CTA may still read its pair; waited for at the end
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 #endif
-  const float ref = finite_or_zero_ref(m), total = s;
+  const float m = sum.m, total = sum.s;
 #endif
-  const float log_prob = known ? (xt - ref) - logf(total) : 0.0f;
+  const float log_prob = known ? log_prob_at(xt, m, total) : 0.0f;
 #if LOG_PROB_OUT
   if (row_ok && part == 0 && t == 0) log_prob_out[r] = log_prob;
 #endif
 #if STATS_OUT
-  if (row_ok && part == 0 && t == 0) stats[r] = make_float2(ref, total);
+  if (row_ok && part == 0 && t == 0) stats[r] = make_float2(m, total);
 #endif
 #if GRADIENT
   SLOPE
-  const float g = known ? slope : 0.0f;
-  // a row that the loss does not depend on is zero whatever its logits hold
-  const bool none = g == 0.0f;
-  const float k = -g / total;
-  const int at = known ? (int)tok : -1;
+  const Slope grad(m, total, slope, known, tok, xt, lead);
   GT* grow = G + r * VOCAB;
-  const unsigned long long minus_ref = pk2(-ref, -ref), log2e = pk2(L2E, L2E), kk = pk2(k, k);
   for (int ck = 0; ck < CHUNKS; ++ck) {
 #if STATS_IN || CHUNKS > 1
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = j0 + (ck * VPT + i) * TPR;
-      if (j < vectors) raw[i] = load_vector(row, lead, j);
-    }
+    load_chunk(mine, row, lead, vectors, j0, ck, raw);
 #endif
+    const int j1 = j0 + ck * (VPT * TPR);
+    if (row_ok && inner_chunk(j1, lead) && !grad.special()) {
+      GT* to = grow + ((long long)j1 * E - lead);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = j0 + (ck * VPT + i) * TPR;
-      if (j >= vectors || !row_ok) continue;
-      const int first = j * E - lead;
-      float f[E];
-      unpack(raw[i], f);
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        float a, b;
-        upk2(mul2(add2(pk2(f[e], f[e + 1]), minus_ref), log2e), a, b);
-        upk2(mul2(pk2(ex2_ftz(a), ex2_ftz(b)), kk), f[e], f[e + 1]);
+      for (int i = 0; i < VPT; ++i) {
+        float f[E];
+        grad.of<false>(raw[i], f);
+        store_vector(to + i * (TPR * E), f);
+        grad.token(grow, j1 + i * TPR);
       }
-      if (none) {
+    } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = 0.0f;
-      } else if (at >= first && at < first + E) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (first + e == at) f[e] += g;
-      }
-      Pack<GT, E> out;
-#pragma unroll
-      for (int e = 0; e < E; ++e) out.v[e] = STORE(f[e]);
-      if (first >= 0 && first + E <= VOCAB) {
-        *reinterpret_cast<Pack<GT, E>*>(grow + first) = out;
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (first + e >= 0 && first + e < VOCAB) grow[first + e] = out.v[e];
+      for (int i = 0; i < VPT; ++i) {
+        const int j = j1 + i * TPR, first = j * E - lead;
+        if (j >= vectors || !row_ok) continue;
+        float f[E];
+        grad.of<true>(raw[i], f);
+        if (first >= 0 && first + E <= VOCAB) store_vector(grow + first, f);
+        else store_edge(grow, first, f);
+        grad.token(grow, j);
       }
     }
   }
@@ -768,28 +862,296 @@ KERNEL(const XT* __restrict__ X, const TT* __restrict__ T, float* __restrict__ l
 }
 )CUDA";
 
+// The same for many long rows: persistent CTAs whose rows pass through a ring of shared-memory slots,
+// filled by bulk copies ahead of use.  A producer warp runs through the rows of the CTA chunk by chunk, into the
+// next row while the consumers are still at this one, so reads go on while the row's threads combine
+// their sums and write the gradient.  The consumers fold each chunk as it arrives (every thread its own
+// running maximum and sum) and keep the last HOLD chunks of the row in their slots; the gradient is
+// computed from those, and then from the row's first chunks, which the producer brings once more (out
+// of L2).  Chunks enter, are released and come back in the one order of the ring.
+const char* kStreamTemplate = R"CUDA(
+#define CHUNK_BYTES (CHUNK * 16)
+#define PER_THREAD (CHUNK / CONSUMERS)
+__device__ __forceinline__ unsigned int shared_at(const void* p) { return (unsigned int)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(shared_at(bar)) : "memory");
+}
+// false when the wait gave up, here or elsewhere in the CTA
+__device__ __forceinline__ bool wait_for(unsigned long long* bar, unsigned int parity, volatile int* gave_up) {
+  const unsigned int a = shared_at(bar);
+  for (unsigned int i = 0; i < (1u << 22); ++i) {
+    unsigned int done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(a), "r"(parity) : "memory");
+    if (done) return true;
+    if (*gave_up) return false;
+  }
+  *gave_up = 1;
+  return false;
+}
+struct Place {   // a position of the ring: slot and the parity of its current use
+  int slot;
+  unsigned int parity;
+  __device__ __forceinline__ void next() { if (++slot == SLOTS) { slot = 0; parity ^= 1u; } }
+};
+struct RowAt {
+  const XT* row;
+  int lead, vectors, chunks, held;
+  // whether every vector of chunk c lies in the row
+  __device__ __forceinline__ bool inner(int c) const {
+    return VOCAB % E == 0 ? (c + 1) * CHUNK <= vectors : c > 0 && (c + 1) * CHUNK < vectors;
+  }
+};
+__device__ __forceinline__ RowAt row_at(const XT* X, long long r) {
+  RowAt w;
+  w.row = X + r * VOCAB;
+  w.lead = (int)(((unsigned long long)w.row & 15ull) / sizeof(XT));
+  w.vectors = (w.lead + VOCAB + E - 1) / E;
+  w.chunks = (w.vectors + CHUNK - 1) / CHUNK;
+  w.held = w.chunks < HOLD ? w.chunks : HOLD;
+  return w;
+}
+// vectors of the buffer that lie inside it altogether; the elements of a last partial one are read singly
+#define WHOLE_VECTORS ((ROWS * (long long)VOCAB) / E)
+
+__device__ __forceinline__ Raw slot_vector(const unsigned char* at) {
+  const uint4 b = *reinterpret_cast<const uint4*>(at);
+  Raw v;
+  v.w[0] = b.x; v.w[1] = b.y; v.w[2] = b.z; v.w[3] = b.w;
+  return v;
+}
+// vector j of a row's first or last chunk: elements outside the row as -inf
+__device__ __forceinline__ Raw edge_vector(const XT* __restrict__ X, const RowAt& w, const unsigned char* at, int j) {
+  Raw v;
+  if (j >= w.vectors) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v.w[q] = NEG_INF_WORD;
+    return v;
+  }
+  v = slot_vector(at);
+  const int first = j * E - w.lead;
+  if (first < 0 || first + E > VOCAB) {
+    const bool whole = (w.row - w.lead - X) / E + j < WHOLE_VECTORS;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool in = first + e >= 0 && first + e < VOCAB;
+#if IN_BITS == 32
+      v.w[e] = !in ? NEG_INF_WORD : whole ? v.w[e] : __float_as_uint(w.row[first + e]);
+#else
+      const unsigned int had = (e & 1) ? v.w[e / 2] >> 16 : v.w[e / 2] & 0xffffu;
+      const unsigned int bits = !in ? NEG_INF_WORD & 0xffffu : whole ? had : (unsigned int)w.row[first + e];
+      v.w[e / 2] = (e & 1) ? (v.w[e / 2] & 0xffffu) | (bits << 16) : (v.w[e / 2] & 0xffff0000u) | bits;
+#endif
+    }
+  }
+  return v;
+}
+
+extern "C" __global__ void __launch_bounds__(CONSUMERS + 32, CTAS_PER_SM)
+KERNEL(const XT* __restrict__ X, const TT* __restrict__ T, float* __restrict__ log_prob_out, float2* __restrict__ stats, GT* __restrict__ G, int* __restrict__ status LEAF_PARAMS) {
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ __align__(8) unsigned long long full[SLOTS], empty[SLOTS];
+  __shared__ float2 cells[2][CONSUMERS / 32];
+  __shared__ int gave_up_cell;
+  volatile int* gave_up = &gave_up_cell;
+  const int t = threadIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (t == 0) {
+    gave_up_cell = 0;
+    for (int i = 0; i < SLOTS; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(shared_at(&full[i])));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(shared_at(&empty[i])), "r"(CONSUMERS / 32));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (warp == CONSUMERS / 32) {
+    if (lane == 0) {
+      Place at{0, 1u};   // the first use of a slot waits for nothing
+      // chunks that will be read again stay in L2 if they can; nothing reads the others again
+      unsigned long long keep, drop;
+      asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+      asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(drop));
+      long long issued = 0;
+      bool ok = true;
+      for (long long r = blockIdx.x; r < ROWS && ok; r += gridDim.x) {
+        const RowAt w = row_at(X, r);
+        const XT* base = w.row - w.lead;
+        const int again = GRADIENT ? w.chunks - w.held : 0;
+        for (int q = 0; q < w.chunks + again; ++q) {
+          const int c = q < w.chunks ? q : q - w.chunks;
+          ok = wait_for(&empty[at.slot], at.parity, gave_up);
+          if (!ok) break;
+          int n = w.vectors - c * CHUNK < CHUNK ? w.vectors - c * CHUNK : CHUNK;
+          if (VOCAB % E != 0 && (base - X) / E + c * CHUNK + n > WHOLE_VECTORS) --n;
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(shared_at(&full[at.slot])), "r"(n * 16) : "memory");
+          if (n > 0)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                         :: "r"(shared_at(ring + at.slot * CHUNK_BYTES)), "l"(base + (long long)c * CHUNK * E), "r"(n * 16), "r"(shared_at(&full[at.slot])), "l"(q < again ? keep : drop) : "memory");
+          at.next();
+          ++issued;
+        }
+      }
+      if (*gave_up) {   // no copy may be in flight when the CTA leaves
+        const long long last = issued < SLOTS ? issued : SLOTS;
+        for (long long q = issued - last; q < issued; ++q) {
+          const unsigned int a = shared_at(&full[q % SLOTS]), parity = (unsigned int)((q / SLOTS) & 1);
+          for (unsigned int i = 0; i < (1u << 22); ++i) {
+            unsigned int done;
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(done) : "r"(a), "r"(parity) : "memory");
+            if (done) break;
+          }
+        }
+        atomicExch(status, 1);
+      }
+    }
+    return;
+  }
+  // Consumers.  After a wait that gave up they go on without waiting (the results are marked invalid by
+  // the status word), so that every warp still meets the others at the row's barrier.
+  Place at{0, 0u};
+  int turn = 0;
+  long long next_tok = (long long)T[blockIdx.x];   // read a row ahead: the token's logit is read at its address
+  for (long long r = blockIdx.x; r < ROWS; r += gridDim.x) {
+    const RowAt w = row_at(X, r);
+    const long long tok = next_tok;
+    if (r + gridDim.x < ROWS) next_tok = (long long)T[r + gridDim.x];
+    const bool known = tok >= 0 && tok < VOCAB;
+    LEAVES
+    const float xt = known ? value_of(w.row[tok]) : 0.0f;
+    Sum sum;
+    Place kept = at;
+    for (int c = 0; c < w.chunks; ++c) {
+      if (c == w.chunks - w.held) kept = at;
+      wait_for(&full[at.slot], at.parity, gave_up);
+      const unsigned char* slot = ring + at.slot * CHUNK_BYTES + t * 16;
+      Raw raw[PER_THREAD];
+      if (w.inner(c)) {
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; ++i) raw[i] = slot_vector(slot + i * (CONSUMERS * 16));
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; ++i) raw[i] = edge_vector(X, w, slot + i * (CONSUMERS * 16), c * CHUNK + i * CONSUMERS + t);
+      }
+      if (!GRADIENT || c < w.chunks - w.held) {
+        __syncwarp();
+        if (lane == 0) arrive(&empty[at.slot]);
+      }
+      at.next();
+      sum.fold(raw);
+    }
+    sum.across_lanes<32>();
+    if (lane == 0) cells[turn][warp] = make_float2(sum.m, sum.s);
+    asm volatile("barrier.sync 1, %0;" :: "n"(CONSUMERS) : "memory");
+    {
+      const float2 mine = cells[turn][lane < CONSUMERS / 32 ? lane : 0];
+      sum.m = mine.x;
+      sum.s = lane < CONSUMERS / 32 ? mine.y : 0.0f;
+      sum.across_lanes<32>();
+    }
+    turn ^= 1;   // the other cells next time: these may still be read
+    const float m = sum.m, total = sum.s;
+    const float log_prob = known ? log_prob_at(xt, m, total) : 0.0f;
+#if LOG_PROB_OUT
+    if (t == 0) log_prob_out[r] = log_prob;
+#endif
+#if STATS_OUT
+    if (t == 0) stats[r] = make_float2(m, total);
+#endif
+#if GRADIENT
+    SLOPE
+    const Slope grad(m, total, slope, known, tok, xt, w.lead);
+    const bool special = grad.special();
+    GT* grow = G + r * VOCAB;
+    for (int q = 0; q < w.chunks; ++q) {
+      const bool held = q < w.held;
+      const int c = held ? w.chunks - w.held + q : q - w.held;
+      const int slot_number = held ? kept.slot : at.slot;
+      if (!held) wait_for(&full[at.slot], at.parity, gave_up);
+      const unsigned char* slot = ring + slot_number * CHUNK_BYTES + t * 16;
+      const int j0 = c * CHUNK + t;
+      const bool inner = w.inner(c);
+      Raw raw[PER_THREAD];
+      if (inner) {
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; ++i) raw[i] = slot_vector(slot + i * (CONSUMERS * 16));
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; ++i) raw[i] = edge_vector(X, w, slot + i * (CONSUMERS * 16), j0 + i * CONSUMERS);
+      }
+      __syncwarp();
+      if (lane == 0) arrive(&empty[slot_number]);
+      if (held) kept.next();
+      else at.next();
+      GT* to = grow + (j0 * E - w.lead);
+      if (inner && !special) {
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; ++i) {
+          float f[E];
+          grad.of<false>(raw[i], f);
+          store_vector(to + i * (CONSUMERS * E), f);
+          grad.token(grow, j0 + i * CONSUMERS);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; ++i) {
+          const int j = j0 + i * CONSUMERS, first = j * E - w.lead;
+          if (j >= w.vectors) continue;
+          const bool whole = first >= 0 && first + E <= VOCAB;
+          float f[E];
+          if (whole && !special) grad.of<false>(raw[i], f);
+          else grad.of<true>(raw[i], f);
+          if (whole) store_vector(to + i * (CONSUMERS * E), f);
+          else store_edge(grow, first, f);
+          grad.token(grow, j);
+        }
+      }
+    }
+#endif
+  }
+}
+)CUDA";
+
 }  // namespace
 
 void emitTokenLogProb(const TokenOp& op, const std::string& name, Plan& plan, const ScheduleOverrides& ov) {
-  if (op.vocab > 0x7fff0000ll) throw PlanError("token log-probabilities over more than 2^31 - 65536 entries are not supported");
+  if (op.vocab > 0x7ff00000ll) throw PlanError("token log-probabilities over more than 2^31 - 2^20 entries are not supported");
   const int in_size = static_cast<int>(dtypeSize(op.logits_dtype)), e = 16 / in_size;
   // aligned vectors that cover a row, wherever it starts
   const int64_t vectors = op.vocab % e == 0 ? op.vocab / e : (op.vocab + 2 * e - 2) / e;
   const bool stats_in = op.stats_in >= 0, gradient = op.grad_slot >= 0;
-  const int most_threads = 512, most_vpt = 8;
+  const int64_t row_bytes = vectors * 16;
+  const int most_threads = 512, most_vpt = 8;   // 64 KB: the row in one CTA's registers, two CTAs per SM
+  // Rows beyond that, with enough of them, pass through shared memory (see kStreamTemplate).  Measured with the
+  // gradient on bf16 4096 x 65536: 203 us, a cluster of two CTAs per row 233 us, chunks read twice 254 us; with 150 rows
+  // the three are equal, with 64 the cluster is the fastest.
+  bool stream = gradient && !stats_in && vectors > most_threads * most_vpt && op.rows >= 2 * ov.sm_count;
   int64_t parts = 1;
+  int tpr = 32;
+  int64_t vpt = most_vpt;
+  int min_blocks = 0;
   if (stats_in) {
     while (parts < 64 && ceilDiv(vectors, parts) > 256 * 4) parts *= 2;
-  } else {
-    // a row that one CTA's registers cannot hold is shared by the CTAs of a cluster; so is any row of more than a few
-    // KB while there are too few rows to fill the GPU
+  } else if (gradient) {
     while (parts < 8 && vectors > parts * most_threads * most_vpt) parts *= 2;
     while (parts < 8 && op.rows * parts * 2 <= 2 * ov.sm_count && vectors >= parts * 2 * 256) parts *= 2;
+  } else {
+    // without a gradient nothing has to be held: a row is split only to fill the GPU (bf16 150 x 131072: 18.5 us in four
+    // parts, 24.6 in one; 600 x 131072: 45 us in four, 37 in one)
+    while (parts < 8 && op.rows * parts * 2 <= 5 * ov.sm_count && vectors >= parts * 2 * 256) parts *= 2;
   }
   const int64_t per = ceilDiv(vectors, parts);
-  int tpr = 32;
-  while (tpr < most_threads && per > static_cast<int64_t>(tpr) * (op.rows * parts <= 2 * ov.sm_count ? 2 : most_vpt)) tpr *= 2;
-  int64_t vpt = std::min<int64_t>(most_vpt, ceilDiv(per, tpr));
+  const bool few = op.rows * parts <= 2 * ov.sm_count;
+  if (!gradient && !few && per > 256 * most_vpt) {
+    // long rows in chunks of 16 KB, six CTAs of 256 threads per SM (bf16 4096 x 32768: 49 us, from registers with 512
+    // threads 53 us; f16 4092 x 50001: 76 us with six CTAs, 84 us with four that read 32 KB at a time)
+    tpr = 256;
+    vpt = 4;
+    min_blocks = 6;
+  } else {
+    while (tpr < most_threads && per > static_cast<int64_t>(tpr) * (few ? 2 : most_vpt)) tpr *= 2;
+    vpt = std::min<int64_t>(most_vpt, ceilDiv(per, tpr));
+  }
   const int64_t chunks = ceilDiv(per, tpr * vpt);
   int rpc = parts == 1 ? std::max(1, 256 / tpr) : 1;
   while (rpc > 1 && rpc / 2 >= op.rows) rpc /= 2;
@@ -811,6 +1173,8 @@ void emitTokenLogProb(const TokenOp& op, const std::string& name, Plan& plan, co
   define(o, "TT", storageTypeOf(op.token_dtype));
   define(o, "GT", storageTypeOf(op.grad_dtype));
   define(o, "STORE(x)", storeConv(op.grad_dtype, "x"));
+  define(o, "OUT_16", op.grad_dtype == DType::f32 ? "0" : "1");
+  define(o, "OUT_16_NAME", op.grad_dtype == DType::bf16 ? "\"bf16\"" : "\"f16\"");
   define(o, "IN_BITS", num(8 * in_size));
   define(o, "IN_BF16", op.logits_dtype == DType::bf16 ? "1" : "0");
   define(o, "E", num(e));
@@ -819,7 +1183,7 @@ void emitTokenLogProb(const TokenOp& op, const std::string& name, Plan& plan, co
   define(o, "TPR", num(tpr));
   define(o, "RPC", num(rpc));
   define(o, "THREADS", num(threads));
-  define(o, "MIN_BLOCKS", num(std::max(1, 1024 / threads)));
+  define(o, "MIN_BLOCKS", num(min_blocks ? min_blocks : std::max(1, 1024 / threads)));
   define(o, "VPT", num(vpt));
   define(o, "CHUNKS", num(chunks));
   define(o, "PARTS", num(parts));
@@ -831,9 +1195,27 @@ void emitTokenLogProb(const TokenOp& op, const std::string& name, Plan& plan, co
   define(o, "LOG_PROB_OUT", op.log_prob_slot >= 0 ? "1" : "0");
   define(o, "GRADIENT", gradient ? "1" : "0");
   define(o, "LEAF_PARAMS", gradient ? slope.params() : "");
-  std::string text = kTokenTemplate;
-  text.replace(text.find("  LEAVES\n"), 9, loads.str());
-  text.replace(text.find("  SLOPE\n"), 8, body.str());
+  // One CTA of 24 warps per SM with a ring of 216 KB for rows of which two such rings hold too little, two CTAs of 16
+  // warps with 96 KB each for shorter ones, whose own latencies then overlap (bf16 4096 x 50001: 174 us with two, 193 us
+  // with one; f32 8192 x 32768: 401 and 348 us; bf16 8192 x 131072: 948 and 711 us).  16-bit logits ask for twice the
+  // arithmetic per byte, so two CTAs serve them up to longer rows.
+  const bool wide_ring = row_bytes >= (in_size == 4 ? 112 : 160) * 1024;
+  const int64_t slots = wide_ring ? 9 : 6, chunk = wide_ring ? 1536 : 1024, consumers = wide_ring ? 768 : 512;
+  const int64_t ctas = wide_ring ? 1 : 2, hold = wide_ring ? 7 : 5;
+  // A gradient of which more than half is computed from logits read again is written past L2, where it would take
+  // their place (f32 2048 x 150000: 522 and 481 us; bf16 8192 x 32768, nothing read again: 182 and 188 us).
+  define(o, "WRITE(p, v)", stream && row_bytes > 2 * hold * chunk * 16 ? "__stcs(p, v)" : "*(p) = (v)");
+  if (stream) {
+    define(o, "SLOTS", num(slots));
+    define(o, "CHUNK", num(chunk));
+    define(o, "CONSUMERS", num(consumers));
+    define(o, "CTAS_PER_SM", num(ctas));
+    define(o, "HOLD", num(hold));
+  }
+  o << kTokenCommon;
+  std::string text = stream ? kStreamTemplate : kTokenTemplate;
+  text.replace(text.find("LEAVES\n"), 7, loads.str());
+  text.replace(text.find("SLOPE\n"), 6, body.str());
   o << text;
   Launch l;
   l.kernel = addKernel(plan, name, "token_log_prob", o.str());
@@ -847,6 +1229,12 @@ void emitTokenLogProb(const TokenOp& op, const std::string& name, Plan& plan, co
   l.args.push_back(or_logits(op.log_prob_slot));
   l.args.push_back(or_logits(stats_in ? op.stats_in : op.stats_out));
   l.args.push_back(or_logits(op.grad_slot));
+  if (stream) {
+    l.args.push_back(slotArg(-2));   // the session's device status word
+    l.grid[0] = static_cast<uint32_t>(std::min<int64_t>(op.rows, ctas * ov.sm_count));
+    l.block[0] = static_cast<uint32_t>(consumers + 32);
+    l.dynamic_smem = static_cast<uint32_t>(slots * chunk * 16);
+  }
   if (gradient)
     for (const LeafRef& leaf : op.slope.leaves) l.args.push_back(slotArg(leaf.slot));
   plan.launches.push_back(l);

@@ -1484,8 +1484,14 @@ class Planner {
 // innermost axis alone), so the operand's inputs would be read once more.  Folding the innermost axis
 // first and the rest in a second, small step changes only the association of the fold, which the
 // kernels' tree-shaped folds change anyway.  Innermost extents below 64 stay as recorded.
+// So do the small folds at the end of a loss on token log-probabilities, whose rows are no row kernel's:
+// two launches would only take longer than one (8192 elements are one CTA's registers).
 static bool foldsInTwoStages(const Program& p, const Operation& op) {
   const Type& in = p.typeOf(op.operands[0]);
+  if (in.elementCount() <= 8192) {
+    for (const Operation& other : p.ops)
+      if (other.kind == Kind::custom_call) return false;
+  }
   long innermost = -1;
   for (size_t i = 0; i < in.rank(); ++i)
     if (in.dims[i].extent != 1) innermost = static_cast<long>(i);

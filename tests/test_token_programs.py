@@ -529,7 +529,7 @@ def test_scatter_add_of_broadcast_and_transposed_updates(gpu_session):
 
 
 ROWS = [((1,), 1), ((1,), 2), ((3,), 7), ((2, 5), 8), ((700,), 9), ((5,), 257), ((3, 3), 1000), ((1,), 4099), ((17,), 33001), ((400,), 5003),
-        ((1,), 131072), ((2,), 70001), ((1,), 300007), ((), 50), ((1300,), 64), ((320,), 32768)]
+        ((1,), 131072), ((2,), 70001), ((1,), 300007), ((), 50), ((1300,), 64), ((320,), 32768), ((297,), 40003), ((300,), 70001)]
 
 
 def logits_and_tokens(dtype, rows, vocab, seed, index="i32"):
@@ -584,8 +584,8 @@ def test_token_log_prob_and_its_gradient(gpu_session, rows, vocab, dtype, index)
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("vocab", [9, 1003, 40000])
-def test_rows_of_infinities_nans_and_lowest_values(gpu_session, dtype, vocab):
+@pytest.mark.parametrize("vocab,copies", [(9, 1), (1003, 1), (40000, 1), (40001, 34)])
+def test_rows_of_infinities_nans_and_lowest_values(gpu_session, dtype, vocab, copies):
     lowest = {"f32": np.finfo(np.float32).min, "f16": -65504.0, "bf16": float(synthetic.bf16_bits_to_f32(np.array([0xff7f], np.uint16))[0])}[dtype]
     rng = np.random.default_rng(4)
     x = exactly(dtype, stored(dtype, rng.standard_normal((9, vocab))))
@@ -597,22 +597,23 @@ def test_rows_of_infinities_nans_and_lowest_values(gpu_session, dtype, vocab):
     x[5, vocab - 1] = np.nan
     x[6] = -lowest
     x[7, 0], x[7, 1:] = -lowest, lowest
-    tok = np.array([1, 2, vocab - 1, 1, 0, 0, 3, 0, vocab], np.int32)
+    n = 9 * copies   # 306 rows of 40001 pass through shared memory, fewer are held in registers
+    x, tok = np.tile(x, (copies, 1)), np.tile(np.array([1, 2, vocab - 1, 1, 0, 0, 3, 0, vocab], np.int32), copies)
     data = stored(dtype, x)
-    specs = [T.spec(dtype, n=9, vocab=vocab), T.spec("i32", n=9), T.spec("f32", n=9)]
+    specs = [T.spec(dtype, n=n, vocab=vocab), T.spec("i32", n=n), T.spec("f32", n=n)]
     want, p, hot, known = log_prob_of(x, tok)
     program = T.define("l", specs, lambda b, a: a[0].token_log_prob(a[1], "vocab").mul(a[2]).sum("n")).grad([0])
     close(run(gpu_session, T.define("l", specs[:2], lambda b, a: a[0].token_log_prob(a[1], "vocab")), [data, tok])[0], want,
           p_error(x) + 4 * U["f32"] * np.abs(np.where(np.isfinite(want), want, 0)))
-    g = np.ones(9, np.float32)
+    g = np.ones(n, np.float32)
     exact = np.where(known[:, None], hot - p, 0)
     with np.errstate(all="ignore"):
         allowed = (p_error(x) + 4 * U["f32"]) * (p + hot) + U[dtype] * np.abs(exact) + TINY[dtype]
     close(run(gpu_session, program, [data, tok, g])[0], exact, allowed)
     # rows whose slope is zero are zero, whatever they hold
-    g[[0, 4, 5]] = 0
+    g.reshape(copies, 9)[:, [0, 4, 5]] = 0
     got = run(gpu_session, program, [data, tok, g])[0]
-    assert np.all(got[[0, 4, 5, 8]] == 0) and np.all(np.isfinite(got))
+    assert np.all(got.reshape(copies, 9, vocab)[:, [0, 4, 5, 8]] == 0) and np.all(np.isfinite(got))
 
 
 @pytest.mark.gpu
