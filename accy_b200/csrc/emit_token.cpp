@@ -54,31 +54,39 @@ struct Pointwise {
     return true;
   }
 
+  // Loads of several rows ahead: the buffers' values as they are stored, `slots` of them per leaf, so that a
+  // row in flight takes no more registers than its bytes; `unpacked` makes node values of slot `a`.
+  bool buffered(int i) const { return nodes[i].op == ENode::Leaf && element(i); }
+  void declareBuffered(int i, std::ostream& o, const std::string& ind, const std::string& slots) const {
+    o << ind << "Pack<" << storageTypeOf(leaves[nodes[i].leaf].dtype) << ", " << vec << "> raw_" << name(i) << "[" << slots << "];\n";
+  }
+  void loadBuffered(int i, std::ostream& o, const std::string& ind) const {
+    const LeafRef& l = leaves[nodes[i].leaf];
+    const std::string L = "L" + num(nodes[i].leaf), st = storageTypeOf(l.dtype), row = indexExpr(extents, l.strides, 0, split, "r");
+    if (vec > 1 && wide(l)) {
+      o << ind << "raw_" << name(i) << "[a * COLUMNS + v] = *reinterpret_cast<const Pack<" << st << ", " << vec << ">*>(" << L << " + " << row << " + c0);\n";
+    } else {
+      o << ind << "#pragma unroll\n" << ind << "for (int e = 0; e < " << vec << "; ++e) raw_" << name(i) << "[a * COLUMNS + v].v[e] = " << L
+        << "[" << row << " + " << indexExpr(extents, l.strides, split, rank(), "(c0 + e)") << "];\n";
+    }
+  }
+  void unpacked(int i, std::ostream& o, const std::string& ind) const {
+    o << ind << ctypeOf(nodes[i].dtype) << " " << name(i) << "[" << vec << "];\n" << ind << "#pragma unroll\n" << ind << "for (int e = 0; e < "
+      << vec << "; ++e) " << name(i) << "[e] = " << loadConv(leaves[nodes[i].leaf].dtype, "raw_" + name(i) + "[a * COLUMNS + v].v[e]") << ";\n";
+  }
+
   void leafLoad(int i, std::ostream& o, const std::string& ind) const {
     const ENode& n = nodes[i];
     const LeafRef& l = leaves[n.leaf];
-    const std::string L = "L" + num(n.leaf), ty = ctypeOf(n.dtype), st = storageTypeOf(l.dtype);
-    const std::string row = indexExpr(extents, l.strides, 0, split, "r");
-    if (!element(i)) {
-      o << ind << "const " << ty << " " << name(i) << " = " << loadConv(l.dtype, L + "[" + row + "]") << ";\n";
-      return;
-    }
-    o << ind << ty << " " << name(i) << "[" << vec << "];\n";
-    if (vec > 1 && wide(l)) {
-      o << ind << "{ const Pack<" << st << ", " << vec << "> p = *reinterpret_cast<const Pack<" << st << ", " << vec << ">*>(" << L
-        << " + " << row << " + c0);\n" << ind << "#pragma unroll\n" << ind << "  for (int e = 0; e < " << vec << "; ++e) " << name(i)
-        << "[e] = " << loadConv(l.dtype, "p.v[e]") << "; }\n";
-    } else {
-      o << ind << "#pragma unroll\n" << ind << "for (int e = 0; e < " << vec << "; ++e) " << name(i) << "[e] = "
-        << loadConv(l.dtype, L + "[" + row + " + " + indexExpr(extents, l.strides, split, rank(), "(c0 + e)") + "]") << ";\n";
-    }
+    o << ind << "const " << ctypeOf(n.dtype) << " " << name(i) << " = "
+      << loadConv(l.dtype, "L" + num(n.leaf) + "[" + indexExpr(extents, l.strides, 0, split, "r") + "]") << ";\n";
   }
 
   void emit(int i, std::ostream& o, const std::string& ind) const {
     const ENode& n = nodes[i];
     const std::string ty = ctypeOf(n.dtype);
     if (i == acc) return;
-    if (n.op == ENode::Leaf) return leafLoad(i, o, ind);
+    if (n.op == ENode::Leaf) return buffered(i) ? unpacked(i, o, ind) : leafLoad(i, o, ind);
     const bool el = element(i);
     std::string value;
     if (n.op == ENode::Const) value = constLiteral(n);
@@ -141,14 +149,88 @@ void define(std::ostream& o, const char* name, const std::string& value) { o << 
 // are then summed by walking the list in equal pieces, whatever the rows' counts are (a padding token may
 // own half of a batch and most tokens own one place).  No sum is an atomic one: the result is the same on
 // every run.  Three launches:
-//   order  one cluster of eight CTAs sorts by least significant digits, its CTAs exchanging digit counts
-//          through distributed shared memory; meanwhile the other CTAs write the rows that no index
-//          names, which for a large vocabulary is most of the traffic;
+//   order  one cluster of eight CTAs sorts by least significant digits and exchanges digit counts through distributed
+//          shared memory.  Meanwhile the other CTAs write the rows that no index names, which for a large
+//          vocabulary is most of the traffic;
 //   sum    one CTA per (piece of the list, block of columns): a thread holds its columns' running sum in
-//          registers (f32 or wider), and writes a row when the run ends.  Runs that cross the ends of a
-//          piece leave partial sums;
+//          registers (f32 or wider) with eight rows in flight, and writes a row when its run ends.  Runs that cross the ends
+//          of a piece leave partial sums;
 //   join   adds the partial sums of the runs that cross, in order.
 // The floor is memory: updates once, rows once.
+const char* kOrderCommon = R"CUDA(
+__device__ __forceinline__ unsigned int row_of(IT x) {
+  const long long v = (long long)x;
+  return v >= 0 && v < EXTENT ? (unsigned int)v : (unsigned int)EXTENT;
+}
+#define PER_LOAD (16 / (int)sizeof(IT))
+
+// The rows that no index names: zeros, or the base's row.  Filler f of FILLERS takes every FILLERS-th group of 32
+// rows, so that frequent (low) numbers, whose rows are not its work, are no filler's alone.  `bits` is a
+// bitmap in shared memory of the named rows of up to WORDS groups.
+#define WORDS 1024
+#define GROUPS ((EXTENT + 31) / 32)
+__device__ __forceinline__ void mark(IT x, unsigned int f, unsigned int first, unsigned int* bits) {
+  const unsigned int v = row_of(x), group = v >> 5, turn = group / FILLERS;
+  if (v < EXTENT && group - turn * FILLERS == f && turn - first < WORDS) atomicOr(&bits[turn - first], 1u << (v & 31));
+}
+__device__ __forceinline__ void fill_rows(const IT* __restrict__ I, OT* __restrict__ out, BASE_PARAM_ unsigned int f, unsigned int* bits) {
+  const int lane = threadIdx.x & 31;
+  for (long long first = 0; first * FILLERS + f < GROUPS; first += WORDS) {
+    long long words = (GROUPS - f + FILLERS - 1) / FILLERS - first;
+    if (words > WORDS) words = WORDS;
+    __syncthreads();
+    for (int w = threadIdx.x; w < words; w += THREADS) bits[w] = 0u;
+    __syncthreads();
+    const long long loads = COUNT / PER_LOAD;
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < loads; i += THREADS) {
+      const Pack<IT, PER_LOAD> some = reinterpret_cast<const Pack<IT, PER_LOAD>*>(I)[i];
+#pragma unroll
+      for (int k = 0; k < PER_LOAD; ++k) mark(some.v[k], f, (unsigned int)first, bits);
+    }
+    for (long long i = loads * PER_LOAD + threadIdx.x; i < COUNT; i += THREADS) mark(I[i], f, (unsigned int)first, bits);
+    __syncthreads();
+    for (int w = threadIdx.x >> 5; w < words; w += THREADS / 32) {
+      const long long row0 = ((first + w) * FILLERS + f) * 32;
+      unsigned int open = ~bits[w];
+      if (EXTENT - row0 < 32) open &= (1u << (EXTENT - row0)) - 1u;
+      while (open) {   // runs of rows without an index: one range of memory each
+        const int from_bit = __ffs(open) - 1;
+        const unsigned int after = ~(open >> from_bit);
+        const int run = after ? __ffs(after) - 1 : 32;
+        open &= run + from_bit >= 32 ? (1u << from_bit) - 1u : ~(((1u << run) - 1u) << from_bit);
+        for (long long p = 0; p < PRE; ++p) {
+          const long long begin = (p * EXTENT + row0 + from_bit) * POST, end = begin + run * POST;
+#if FROM_ZEROS
+          // whole 16-byte units, the elements before and after them one by one
+          constexpr int U = 16 / (int)sizeof(OT);
+          long long from = (begin + U - 1) / U * U, to = end / U * U;
+          if (from > to) from = to = end;
+          if (begin + lane < from) out[begin + lane] = (OT)0;
+          if (to + lane < end) out[to + lane] = (OT)0;
+          uint4* at = reinterpret_cast<uint4*>(out + from) + lane;
+          uint4* const stop = reinterpret_cast<uint4*>(out + to);
+#pragma unroll 1
+          for (; at + 7 * 32 < stop; at += 8 * 32) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) at[u * 32] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          for (; at < stop; at += 32) *at = make_uint4(0u, 0u, 0u, 0u);
+#else
+          for (long long q = begin + lane * FVEC; q < end; q += 32 * FVEC) {
+            Pack<OT, FVEC> o;
+#pragma unroll
+            for (int e = 0; e < FVEC; ++e) o.v[e] = FILL_VALUE(q + e);
+            *reinterpret_cast<Pack<OT, FVEC>*>(out + q) = o;
+          }
+#endif
+        }
+      }
+    }
+  }
+}
+)CUDA";
+
 const char* kOrderTemplate = R"CUDA(
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
@@ -160,73 +242,54 @@ __device__ __forceinline__ unsigned int peer_word(const unsigned int* p, unsigne
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(b) : "memory");
   return v;
 }
-__device__ __forceinline__ unsigned int row_of(IT x) {
-  const long long v = (long long)x;
-  return v >= 0 && v < EXTENT ? (unsigned int)v : (unsigned int)EXTENT;
-}
-
-// Rows [lo, hi) that no index names: zeros, or the base's row.
-__device__ __forceinline__ void fill_rows(const IT* __restrict__ I, OT* __restrict__ out, BASE_PARAM_ long long lo, long long hi, unsigned int* bits) {
-  for (long long at = lo; at < hi; at += FILL_ROWS) {
-    const long long end = at + FILL_ROWS < hi ? at + FILL_ROWS : hi;
-    __syncthreads();
-    for (int w = threadIdx.x; w < FILL_ROWS / 32; w += THREADS) bits[w] = 0u;
-    __syncthreads();
-#pragma unroll 4
-    for (long long i = threadIdx.x; i < COUNT; i += THREADS) {
-      const long long v = (long long)I[i];
-      if (v >= at && v < end) atomicOr(&bits[(v - at) >> 5], 1u << ((v - at) & 31));
-    }
-    __syncthreads();
-    const long long vectors = (end - at) * (POST / FVEC);
-    for (long long p = 0; p < PRE; ++p) {
-      for (long long q = threadIdx.x; q < vectors; q += THREADS) {
-        const long long v = q / (POST / FVEC), c = (q - v * (POST / FVEC)) * FVEC;
-        if (bits[v >> 5] >> (v & 31) & 1u) continue;
-        const long long off = (p * EXTENT + at + v) * POST + c;
-        Pack<OT, FVEC> o;
-#pragma unroll
-        for (int e = 0; e < FVEC; ++e) o.v[e] = FILL_VALUE(off + e);
-        *reinterpret_cast<Pack<OT, FVEC>*>(out + off) = o;
-      }
-    }
-  }
-}
-
-extern "C" __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(THREADS)
+// Keys are taken BATCH at a time per lane, all of a batch's loads before its first use.  Where a lane has no
+// more than one batch, the places found while counting are kept for the second loop.
+#define BATCH 8
+#define ONE_BATCH (SLICE <= BATCH * 32)
+extern "C" __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(THREADS, 2)
 KERNEL(const IT* __restrict__ I, unsigned int* key_a, unsigned int* pos_a, unsigned int* key_b, unsigned int* pos_b, OT* __restrict__ out BASE_PARAM) {
-  __shared__ unsigned int hist[WARPS][RADIX];
-  __shared__ unsigned int total[RADIX], start[RADIX], wsum[WARPS], bits[FILL_ROWS / 32];
+  __shared__ unsigned int pool[WARPS * RADIX > WORDS ? WARPS * RADIX : WORDS];
+  __shared__ unsigned int total[RADIX], start[RADIX], wsum[WARPS];
   if (blockIdx.x >= 8) {   // whole clusters take this branch
-    const long long f = blockIdx.x - 8, per = (EXTENT + FILLERS - 1) / FILLERS;
-    const long long lo = f * per, hi = lo + per < EXTENT ? lo + per : EXTENT;
-    fill_rows(I, out, BASE_ARG_ lo, hi, bits);
+    fill_rows(I, out, BASE_ARG_ blockIdx.x - 8, pool);
     return;
   }
+  unsigned int (*hist)[RADIX] = reinterpret_cast<unsigned int (*)[RADIX]>(pool);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned int cta = blockIdx.x;
-  // every warp owns one run of places, in order: that is what keeps the sort stable
-  const long long slice = ((COUNT + 8 * WARPS * 32 - 1) / (8 * WARPS * 32)) * 32;
-  const long long w0 = ((long long)cta * WARPS + warp) * slice, w1 = w0 + slice < COUNT ? w0 + slice : COUNT;
+  // every warp owns one run of SLICE places, in order: that is what keeps the sort stable
+  const long long w0 = ((long long)cta * WARPS + warp) * SLICE, w1 = w0 + SLICE < COUNT ? w0 + SLICE : COUNT;
   for (int pass = 0; pass < PASSES; ++pass) {
     // the last pass writes the (a) arrays
     const bool to_a = ((PASSES - 1 - pass) & 1) == 0;
     const unsigned int *ks = to_a ? key_b : key_a, *ps = to_a ? pos_b : pos_a;
     unsigned int *kd = to_a ? key_a : key_b, *pd = to_a ? pos_a : pos_b;
     const int shift = pass * DIGIT_BITS;
+    unsigned int k[BATCH], place[BATCH];
     for (int d = threadIdx.x; d < WARPS * RADIX; d += THREADS) (&hist[0][0])[d] = 0u;
     __syncthreads();
-    for (long long i = w0 + lane; i - lane < w1; i += 32) {
-      const bool in = i < w1;
-      unsigned int d = RADIX;
-      if (in) d = ((pass == 0 ? row_of(I[i]) : __ldcg(ks + i)) >> shift) & (RADIX - 1);
-      const unsigned int peers = __match_any_sync(0xffffffffu, d);
-      if (in && lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
-      __syncwarp();
+    for (long long b = w0; b < w1; b += BATCH * 32) {
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const long long i = b + j * 32 + lane;
+        k[j] = i < w1 ? (pass == 0 ? row_of(I[i]) : __ldcg(ks + i)) : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        if (b + j * 32 >= w1) break;
+        const bool in = b + j * 32 + lane < w1;
+        const unsigned int d = in ? (k[j] >> shift) & (RADIX - 1) : RADIX;
+        const unsigned int peers = __match_any_sync(0xffffffffu, d);
+        if (in) place[j] = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
+        __syncwarp();
+        if (in && lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
+        __syncwarp();
+      }
     }
     __syncthreads();
     if (threadIdx.x < RADIX) {
       unsigned int sum = 0u;
+#pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         const unsigned int n = hist[w][threadIdx.x];
         hist[w][threadIdx.x] = sum;
@@ -258,91 +321,113 @@ KERNEL(const IT* __restrict__ I, unsigned int* key_a, unsigned int* pos_a, unsig
       start[threadIdx.x] = ex + before;
     }
     __syncthreads();
-    for (long long i = w0 + lane; i - lane < w1; i += 32) {
-      const bool in = i < w1;
-      unsigned int k = 0u, ps_i = 0u, d = RADIX;
-      if (in) {
-        k = pass == 0 ? row_of(I[i]) : __ldcg(ks + i);
-        ps_i = pass == 0 ? (unsigned int)i : __ldcg(ps + i);
-        d = (k >> shift) & (RADIX - 1);
+    for (long long b = w0; b < w1; b += BATCH * 32) {
+      unsigned int from[BATCH];
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const long long i = b + j * 32 + lane;
+        if (!ONE_BATCH) k[j] = i < w1 ? (pass == 0 ? row_of(I[i]) : __ldcg(ks + i)) : 0u;
+        from[j] = i < w1 && pass > 0 ? __ldcg(ps + i) : (unsigned int)i;
       }
-      const unsigned int peers = __match_any_sync(0xffffffffu, d);
-      if (in) {
-        const unsigned int to = start[d] + hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
-        kd[to] = k;
-        pd[to] = ps_i;
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        if (b + j * 32 >= w1) break;
+        const bool in = b + j * 32 + lane < w1;
+        const unsigned int d = in ? (k[j] >> shift) & (RADIX - 1) : RADIX;
+        if (ONE_BATCH) {
+          // hist holds what this CTA's earlier warps have of the digit
+          if (in) place[j] += hist[warp][d];
+        } else {
+          const unsigned int peers = __match_any_sync(0xffffffffu, d);
+          if (in) place[j] = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
+          __syncwarp();
+          if (in && lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
+          __syncwarp();
+        }
+        if (in) {
+          kd[start[d] + place[j]] = k[j];
+          pd[start[d] + place[j]] = from[j];
+        }
       }
-      __syncwarp();
-      if (in && lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
-      __syncwarp();
     }
     cluster_sync();   // the lists are complete, and nobody reads this pass's counts any more
   }
 }
 )CUDA";
 
+// A thread has COLUMNS vectors of VEC columns, THREADS vectors apart: where rows are too badly aligned for 16-byte
+// accesses it takes that many narrower ones, so that what a row costs besides (its key, its place, the end of
+// its run) is spread over as much data.
 const char* kSumHead = R"CUDA(
-__device__ __forceinline__ void write_row(OT* __restrict__ out, BASE_PARAM_ long long off, const VT (&sum)[VEC]) {
+// p * EXTENT + k and the like fit 32 bits in all but the largest calls; a 32-bit factor makes the offset one instruction
+#define OFFSET(row) ((long long)(ROW_T)(row) * POST)
+__device__ __forceinline__ void write_row(OT* __restrict__ out, BASE_PARAM_ long long off, const VT* sum) {
   Pack<OT, VEC> o;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) o.v[e] = WITH_BASE(off + e, sum[e]);
   *reinterpret_cast<Pack<OT, VEC>*>(out + off) = o;
 }
+#define EACH_COLUMN(v, c0) _Pragma("unroll") for (int v = 0; v < COLUMNS; ++v) if (const long long c0 = column + v * (THREADS * VEC); c0 < POST)
 )CUDA";
 
 const char* kSumBody = R"CUDA(
-  __shared__ unsigned int key[PIECE + 2], pos[PIECE];
+  __shared__ unsigned int key[PIECE + AHEAD + 2], pos[PIECE + AHEAD];
   const long long begin = (long long)blockIdx.x * PIECE;
   const int n = COUNT - begin < PIECE ? (int)(COUNT - begin) : PIECE;
   // key[0] and key[n + 1] are the neighbours' keys; EXTENT + 1 stands for none
-  for (int i = threadIdx.x; i < n + 2; i += THREADS) {
+  for (int i = threadIdx.x; i < PIECE + AHEAD + 2; i += THREADS) {
     const long long at = begin + i - 1;
-    key[i] = at >= 0 && at < COUNT ? keys[at] : (unsigned int)EXTENT + 1u;
-    if (i < n) pos[i] = places[begin + i];
+    key[i] = i < n + 2 && at >= 0 && at < COUNT ? keys[at] : (unsigned int)EXTENT + 1u;
+    if (i < PIECE + AHEAD) pos[i] = i < n ? places[begin + i] : 0u;
   }
   __syncthreads();
-  const long long c0 = ((long long)blockIdx.y * THREADS + threadIdx.x) * VEC;
-  if (c0 >= POST) return;
-  const long long p = blockIdx.z;
-  VT sum[VEC];
+  const long long column = ((long long)blockIdx.y * (THREADS * COLUMNS) + threadIdx.x) * VEC;
+  const ROW_T p_index = (ROW_T)blockIdx.z * (ROW_T)COUNT, p_row = (ROW_T)blockIdx.z * (ROW_T)EXTENT;
+  VT sum[COLUMNS * VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) sum[e] = 0;
+  for (int e = 0; e < COLUMNS * VEC; ++e) sum[e] = 0;
   bool first = true;   // the run that starts this piece
   for (int i = 0; i < n; i += AHEAD) {
-    VT u[AHEAD][VEC];
+    unsigned int k[AHEAD + 1];
+#pragma unroll
+    for (int a = 0; a <= AHEAD; ++a) k[a] = key[i + a + 1];
+    DECLARE
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      if (i + a >= n || key[i + a + 1] >= (unsigned int)EXTENT) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) u[a][e] = 0;
-        continue;
-      }
-      const long long r = p * COUNT + pos[i + a];
+      if (i + a >= n || k[a] >= (unsigned int)EXTENT) break;
+      const ROW_T r = p_index + pos[i + a];
       (void)r;
-      UPDATE
+      EACH_COLUMN(v, c0) {
+        LOAD
+      }
     }
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
       if (i + a >= n) break;
-      const unsigned int k = key[i + a + 1];
-      if (k >= (unsigned int)EXTENT) return;   // indices outside the axis come last
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e] = sum[e] + u[a][e];
-      const bool last = i + a + 1 == n;
-      if (!last && key[i + a + 2] == k) continue;
-      // the run ends here, or the piece does
-      const bool from_before = first && key[0] == k, goes_on = last && key[n + 1] == k;
-      if (from_before || goes_on) {
-        Pack<VT, VEC> part;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) part.v[e] = sum[e];
-        *reinterpret_cast<Pack<VT, VEC>*>(partial + ((p * PIECES + blockIdx.x) * 2 + (from_before ? 0 : 1)) * POST + c0) = part;
-      } else {
-        write_row(out, BASE_ARG_ (p * EXTENT + k) * POST + c0, sum);
+      if (k[a] >= (unsigned int)EXTENT) return;   // indices outside the axis come last
+      const ROW_T r = p_index + pos[i + a];
+      (void)r;
+      EACH_COLUMN(v, c0) {
+        UPDATE
       }
+      const bool last = i + a + 1 == n;
+      if (!last && k[a + 1] == k[a]) continue;
+      // the run ends here, or the piece does
+      const bool from_before = first && key[0] == k[a], goes_on = last && k[a + 1] == k[a];
       first = false;
+      if (from_before || goes_on) {
+        VT* to = partial + (((long long)blockIdx.z * PIECES + blockIdx.x) * 2 + (from_before ? 0 : 1)) * POST;
+        EACH_COLUMN(v, c0) {
+          Pack<VT, VEC> part;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e] = 0;
+          for (int e = 0; e < VEC; ++e) part.v[e] = sum[v * VEC + e];
+          *reinterpret_cast<Pack<VT, VEC>*>(to + c0) = part;
+        }
+      } else {
+        EACH_COLUMN(v, c0) write_row(out, BASE_ARG_ OFFSET(p_row + k[a]) + c0, sum + v * VEC);
+      }
+#pragma unroll
+      for (int e = 0; e < COLUMNS * VEC; ++e) sum[e] = 0;
     }
   }
 }
@@ -352,9 +437,9 @@ const char* kJoinBody = R"CUDA(
   const long long piece = blockIdx.x, begin = piece * PIECE, end = begin + PIECE;
   if (end >= COUNT) return;
   const unsigned int k = keys[end - 1];
+  const unsigned int next = keys[end], before = begin > 0 ? keys[begin - 1] : (unsigned int)EXTENT + 1u;
   // the run at the end of this piece goes on, and began in it
-  if (k >= (unsigned int)EXTENT || keys[end] != k) return;
-  if (begin > 0 && keys[begin - 1] == k) return;
+  if (k >= (unsigned int)EXTENT || next != k || before == k) return;
   // how many of the following pieces begin with it: they are next to each other
   long long more = 0;
   for (;;) {
@@ -373,13 +458,22 @@ const char* kJoinBody = R"CUDA(
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[e] = part.v[e];
   }
-#pragma unroll 8
-  for (long long m = 1; m <= more; ++m) {
-    const Pack<VT, VEC> part = *reinterpret_cast<const Pack<VT, VEC>*>(from + m * 2 * POST);
+#pragma unroll 1
+  for (long long m = 1; m <= more; m += AHEAD) {
+    Pack<VT, VEC> part[AHEAD];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) sum[e] = sum[e] + part.v[e];
+    for (int a = 0; a < AHEAD; ++a) {
+      if (m + a > more) break;
+      part[a] = *reinterpret_cast<const Pack<VT, VEC>*>(from + (m + a) * 2 * POST);
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (m + a > more) break;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] = sum[e] + part[a].v[e];
+    }
   }
-  write_row(out, BASE_ARG_ (p * EXTENT + k) * POST + c0, sum);
+  write_row(out, BASE_ARG_ OFFSET((ROW_T)p * (ROW_T)EXTENT + k) + c0, sum);
 }
 )CUDA";
 
@@ -396,16 +490,23 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
   while (fvec > 1 && s.post % fvec != 0) fvec /= 2;
   int bits = 1;
   while ((int64_t{1} << bits) < s.extent + 1) ++bits;
-  const int passes = static_cast<int>(ceilDiv(bits, 8)), digit_bits = static_cast<int>(ceilDiv(bits, passes));
+  const int passes = static_cast<int>(ceilDiv(bits, 9)), digit_bits = static_cast<int>(ceilDiv(bits, passes));
   const int64_t out_bytes = s.pre * s.extent * s.post * static_cast<int64_t>(dtypeSize(s.out_dtype));
-  const int64_t fillers = 8 * std::max<int64_t>(1, std::min<int64_t>(ceilDiv(out_bytes, 8 * 65536), ceilDiv(2 * ov.sm_count, 8)));
+  // Fillers in whole clusters, no more than write 64 KB each.  Clusters are placed two CTAs to an SM before all SMs have
+  // one, so it takes several per SM to use them all (131072 rows of 8 KB: 346 us for all three launches with 17 clusters,
+  // 297 with 26, 268 with 71, 281 with 140).
+  const int64_t fillers = 8 * std::max<int64_t>(1, std::min<int64_t>(ceilDiv(out_bytes, 8 * 65536), (ov.sm_count - 4) / 2));
 
-  const int threads = static_cast<int>(std::min<int64_t>(256, ceilDiv(ceilDiv(s.post, vec), 32) * 32));
-  const int64_t blocks = ceilDiv(s.post, static_cast<int64_t>(threads) * vec);
+  const int columns = static_cast<int>(std::min<int64_t>(widest / vec, ceilDiv(s.post, 32 * vec)));
+  const int64_t lanes = ceilDiv(s.post, vec * columns);   // threads that a row takes
+  const int64_t blocks = ceilDiv(lanes, 256);
+  const int threads = static_cast<int>(ceilDiv(ceilDiv(lanes, blocks), 32) * 32);
   if (blocks > 65535) throw PlanError("scatter_add rows are too long");
-  // about eight CTAs per SM; longer pieces leave fewer partial sums
+  // At least four CTAs per SM while pieces are worth having: a piece is walked one place after the other, about 0.15 us
+  // each, and each piece may leave two partial sums (bf16 16384 places of 4096: 104 us in pieces of 8, 86 of 32, 96 of 128;
+  // f32 9999 of 513: 35, 31 and 51; bf16 2048 of 2048: 35, 41 and 68).
   int64_t piece = 8;
-  while (piece < 128 && ceilDiv(s.count, piece * 2) * blocks * s.pre >= 8 * ov.sm_count) piece *= 2;
+  while (piece < 128 && ceilDiv(s.count, piece * 2) * blocks * s.pre >= 4 * ov.sm_count) piece *= 2;
   const int64_t pieces = ceilDiv(s.count, piece);
 
   const int key_a = scratchSlot(plan, s.count * 4), pos_a = scratchSlot(plan, s.count * 4);
@@ -436,14 +537,15 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
     head(o);
     define(o, "KERNEL", name + "_order");
     define(o, "THREADS", "512");
+    define(o, "FROM_ZEROS", s.base_slot < 0 ? "1" : "0");
+    define(o, "FVEC", num(fvec));
+    define(o, "FILLERS", num(fillers) + "u");
     define(o, "WARPS", "16");
     define(o, "PASSES", num(passes));
     define(o, "DIGIT_BITS", num(digit_bits));
     define(o, "RADIX", num(1 << digit_bits));
-    define(o, "FILLERS", num(fillers) + "ll");
-    define(o, "FILL_ROWS", "32768");
-    define(o, "FVEC", num(fvec));
-    o << kOrderTemplate;
+    define(o, "SLICE", num(ceilDiv(s.count, 8 * 16 * 32) * 32));
+    o << kOrderCommon << kOrderTemplate;
     Launch l;
     l.kernel = addKernel(plan, name + "_order", "scatter_add", o.str());
     l.grid[0] = static_cast<uint32_t>(8 + fillers);
@@ -453,18 +555,20 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
     if (s.base_slot >= 0) l.args.push_back(slotArg(s.base_slot));
     plan.launches.push_back(l);
   }
-  auto sumHead = [&](std::ostream& o, const char* kernel, const std::string& more) {
+  auto sumHead = [&](std::ostream& o, const char* kernel, const std::string& more, int threads, int vec, int columns, int ahead) {
     head(o);
+    define(o, "COLUMNS", num(columns));
+    define(o, "ROW_T", s.pre * std::max(s.extent, s.count) < (int64_t{1} << 32) ? "unsigned int" : "long long");
     define(o, "THREADS", num(threads));
     define(o, "VEC", num(vec));
     define(o, "PIECE", num(piece));
     define(o, "PIECES", num(pieces) + "ll");
-    define(o, "AHEAD", "4");
+    define(o, "AHEAD", num(ahead));
     o << kSumHead << "extern \"C\" __global__ void __launch_bounds__(" << threads << ") " << name << kernel
       << "(const unsigned int* __restrict__ keys, const unsigned int* __restrict__ places, " << vt << "* __restrict__ partial, " << ot
       << "* __restrict__ out BASE_PARAM" << more << ") {\n";
   };
-  auto sumLaunch = [&](int kernel, const char* what) {
+  auto sumLaunch = [&](int kernel, const char* what, int threads, int64_t blocks) {
     Launch l;
     l.kernel = kernel;
     l.grid[0] = static_cast<uint32_t>(pieces);
@@ -478,22 +582,36 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
   };
   {
     Pointwise g{s.updates.nodes, s.updates.leaves, s.updates.extents, s.updates.split, vec, -1, "", "n"};
-    std::ostringstream o, update;
-    for (size_t i = 0; i < g.nodes.size(); ++i) g.emit(static_cast<int>(i), update, "      ");
-    update << "#pragma unroll\n      for (int e = 0; e < VEC; ++e) u[a][e] = " << g.at(s.result) << ";\n";
-    sumHead(o, "_sum", g.params());
+    std::ostringstream o, declare, load, update;
+    for (size_t i = 0; i < g.nodes.size(); ++i) {
+      const int n = static_cast<int>(i);
+      if (g.buffered(n)) {
+        g.declareBuffered(n, declare, "    ", "AHEAD * COLUMNS");
+        g.loadBuffered(n, load, "      ");
+      }
+      g.emit(n, update, "      ");
+    }
+    update << "#pragma unroll\n      for (int e = 0; e < VEC; ++e) sum[v * VEC + e] = sum[v * VEC + e] + " << g.at(s.result) << ";\n";
+    sumHead(o, "_sum", g.params(), threads, vec, columns, 8);
     std::string body = kSumBody;
-    body.replace(body.find("UPDATE"), 6, update.str());
+    body.replace(body.find("DECLARE"), 7, declare.str());
+    body.replace(body.find("LOAD\n"), 5, load.str());
+    body.replace(body.find("UPDATE\n"), 7, update.str());
     o << body;
-    Launch l = sumLaunch(addKernel(plan, name + "_sum", "scatter_add", o.str()), " sum");
+    Launch l = sumLaunch(addKernel(plan, name + "_sum", "scatter_add", o.str()), " sum", threads, blocks);
     for (const LeafRef& leaf : s.updates.leaves) l.args.push_back(slotArg(leaf.slot));
     plan.launches.push_back(l);
   }
   if (pieces > 1) {
+    // partial sums are f32 or f64: 16 bytes of them per thread, sixteen in flight
+    const int join_vec = std::min(vec, wide ? 2 : 4);
+    const int64_t join_lanes = ceilDiv(s.post, join_vec), join_blocks = ceilDiv(join_lanes, 256);
+    const int join_threads = static_cast<int>(ceilDiv(ceilDiv(join_lanes, join_blocks), 32) * 32);
+    if (join_blocks > 65535) throw PlanError("scatter_add rows are too long");
     std::ostringstream o;
-    sumHead(o, "_join", "");
+    sumHead(o, "_join", "", join_threads, join_vec, 1, 16);
     o << "  (void)places;\n" << kJoinBody;
-    plan.launches.push_back(sumLaunch(addKernel(plan, name + "_join", "scatter_add", o.str()), " join"));
+    plan.launches.push_back(sumLaunch(addKernel(plan, name + "_join", "scatter_add", o.str()), " join", join_threads, join_blocks));
   }
 }
 
