@@ -247,7 +247,7 @@ __device__ __forceinline__ unsigned int peer_word(const unsigned int* p, unsigne
 #define BATCH 8
 #define ONE_BATCH (SLICE <= BATCH * 32)
 extern "C" __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(THREADS, 2)
-KERNEL(const IT* __restrict__ I, unsigned int* key_a, unsigned int* pos_a, unsigned int* key_b, unsigned int* pos_b, OT* __restrict__ out BASE_PARAM) {
+KERNEL(const IT* __restrict__ I, uint2* list_a, uint2* list_b, OT* __restrict__ out BASE_PARAM) {
   __shared__ unsigned int pool[WARPS * RADIX > WORDS ? WARPS * RADIX : WORDS];
   __shared__ unsigned int total[RADIX], start[RADIX], wsum[WARPS];
   if (blockIdx.x >= 8) {   // whole clusters take this branch
@@ -260,27 +260,28 @@ KERNEL(const IT* __restrict__ I, unsigned int* key_a, unsigned int* pos_a, unsig
   // every warp owns one run of SLICE places, in order: that is what keeps the sort stable
   const long long w0 = ((long long)cta * WARPS + warp) * SLICE, w1 = w0 + SLICE < COUNT ? w0 + SLICE : COUNT;
   for (int pass = 0; pass < PASSES; ++pass) {
-    // the last pass writes the (a) arrays
+    // the last pass writes list a
     const bool to_a = ((PASSES - 1 - pass) & 1) == 0;
-    const unsigned int *ks = to_a ? key_b : key_a, *ps = to_a ? pos_b : pos_a;
-    unsigned int *kd = to_a ? key_a : key_b, *pd = to_a ? pos_a : pos_b;
+    const uint2* from = to_a ? list_b : list_a;
+    uint2* to = to_a ? list_a : list_b;
     const int shift = pass * DIGIT_BITS;
-    unsigned int k[BATCH], place[BATCH];
+    uint2 k[BATCH];   // key and place
+    unsigned int offset[BATCH];
     for (int d = threadIdx.x; d < WARPS * RADIX; d += THREADS) (&hist[0][0])[d] = 0u;
     __syncthreads();
     for (long long b = w0; b < w1; b += BATCH * 32) {
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
         const long long i = b + j * 32 + lane;
-        k[j] = i < w1 ? (pass == 0 ? row_of(I[i]) : __ldcg(ks + i)) : 0u;
+        if (i < w1) k[j] = pass == 0 ? make_uint2(row_of(I[i]), (unsigned int)i) : __ldcg(from + i);
       }
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
         if (b + j * 32 >= w1) break;
         const bool in = b + j * 32 + lane < w1;
-        const unsigned int d = in ? (k[j] >> shift) & (RADIX - 1) : RADIX;
+        const unsigned int d = in ? (k[j].x >> shift) & (RADIX - 1) : RADIX;
         const unsigned int peers = __match_any_sync(0xffffffffu, d);
-        if (in) place[j] = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
+        if (in) offset[j] = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
         __syncwarp();
         if (in && lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
         __syncwarp();
@@ -322,35 +323,30 @@ KERNEL(const IT* __restrict__ I, unsigned int* key_a, unsigned int* pos_a, unsig
     }
     __syncthreads();
     for (long long b = w0; b < w1; b += BATCH * 32) {
-      unsigned int from[BATCH];
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
         const long long i = b + j * 32 + lane;
-        if (!ONE_BATCH) k[j] = i < w1 ? (pass == 0 ? row_of(I[i]) : __ldcg(ks + i)) : 0u;
-        from[j] = i < w1 && pass > 0 ? __ldcg(ps + i) : (unsigned int)i;
+        if (!ONE_BATCH && i < w1) k[j] = pass == 0 ? make_uint2(row_of(I[i]), (unsigned int)i) : __ldcg(from + i);
       }
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
         if (b + j * 32 >= w1) break;
         const bool in = b + j * 32 + lane < w1;
-        const unsigned int d = in ? (k[j] >> shift) & (RADIX - 1) : RADIX;
+        const unsigned int d = in ? (k[j].x >> shift) & (RADIX - 1) : RADIX;
         if (ONE_BATCH) {
           // hist holds what this CTA's earlier warps have of the digit
-          if (in) place[j] += hist[warp][d];
+          if (in) offset[j] += hist[warp][d];
         } else {
           const unsigned int peers = __match_any_sync(0xffffffffu, d);
-          if (in) place[j] = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
+          if (in) offset[j] = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
           __syncwarp();
           if (in && lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
           __syncwarp();
         }
-        if (in) {
-          kd[start[d] + place[j]] = k[j];
-          pd[start[d] + place[j]] = from[j];
-        }
+        if (in) to[start[d] + offset[j]] = k[j];
       }
     }
-    cluster_sync();   // the lists are complete, and nobody reads this pass's counts any more
+    cluster_sync();   // the list is complete, and nobody reads this pass's counts any more
   }
 }
 )CUDA";
@@ -371,14 +367,15 @@ __device__ __forceinline__ void write_row(OT* __restrict__ out, BASE_PARAM_ long
 )CUDA";
 
 const char* kSumBody = R"CUDA(
-  __shared__ unsigned int key[PIECE + AHEAD + 2], pos[PIECE + AHEAD];
+  __shared__ unsigned int key[PIECE + AHEAD + 2], pos[PIECE + AHEAD + 2];   // of place i at i + 1
   const long long begin = (long long)blockIdx.x * PIECE;
   const int n = COUNT - begin < PIECE ? (int)(COUNT - begin) : PIECE;
   // key[0] and key[n + 1] are the neighbours' keys; EXTENT + 1 stands for none
   for (int i = threadIdx.x; i < PIECE + AHEAD + 2; i += THREADS) {
     const long long at = begin + i - 1;
-    key[i] = i < n + 2 && at >= 0 && at < COUNT ? keys[at] : (unsigned int)EXTENT + 1u;
-    if (i < PIECE + AHEAD) pos[i] = i < n ? places[begin + i] : 0u;
+    const uint2 one = i < n + 2 && at >= 0 && at < COUNT ? list[at] : make_uint2((unsigned int)EXTENT + 1u, 0u);
+    key[i] = one.x;
+    pos[i] = one.y;
   }
   __syncthreads();
   const long long column = ((long long)blockIdx.y * (THREADS * COLUMNS) + threadIdx.x) * VEC;
@@ -395,7 +392,7 @@ const char* kSumBody = R"CUDA(
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
       if (i + a >= n || k[a] >= (unsigned int)EXTENT) break;
-      const ROW_T r = p_index + pos[i + a];
+      const ROW_T r = p_index + pos[i + a + 1];
       (void)r;
       EACH_COLUMN(v, c0) {
         LOAD
@@ -405,7 +402,7 @@ const char* kSumBody = R"CUDA(
     for (int a = 0; a < AHEAD; ++a) {
       if (i + a >= n) break;
       if (k[a] >= (unsigned int)EXTENT) return;   // indices outside the axis come last
-      const ROW_T r = p_index + pos[i + a];
+      const ROW_T r = p_index + pos[i + a + 1];
       (void)r;
       EACH_COLUMN(v, c0) {
         UPDATE
@@ -436,15 +433,14 @@ const char* kSumBody = R"CUDA(
 const char* kJoinBody = R"CUDA(
   const long long piece = blockIdx.x, begin = piece * PIECE, end = begin + PIECE;
   if (end >= COUNT) return;
-  const unsigned int k = keys[end - 1];
-  const unsigned int next = keys[end], before = begin > 0 ? keys[begin - 1] : (unsigned int)EXTENT + 1u;
+  const unsigned int k = list[end - 1].x, next = list[end].x, before = begin > 0 ? list[begin - 1].x : (unsigned int)EXTENT + 1u;
   // the run at the end of this piece goes on, and began in it
   if (k >= (unsigned int)EXTENT || next != k || before == k) return;
   // how many of the following pieces begin with it: they are next to each other
   long long more = 0;
   for (;;) {
     const long long at = (piece + 1 + more + threadIdx.x) * PIECE;
-    const int here = __syncthreads_count(at < COUNT && keys[at] == k);
+    const int here = __syncthreads_count(at < COUNT && list[at].x == k);
     more += here;
     if (here < THREADS) break;
   }
@@ -509,8 +505,7 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
   while (piece < 128 && ceilDiv(s.count, piece * 2) * blocks * s.pre >= 4 * ov.sm_count) piece *= 2;
   const int64_t pieces = ceilDiv(s.count, piece);
 
-  const int key_a = scratchSlot(plan, s.count * 4), pos_a = scratchSlot(plan, s.count * 4);
-  const int key_b = scratchSlot(plan, s.count * 4), pos_b = scratchSlot(plan, s.count * 4);
+  const int list_a = scratchSlot(plan, s.count * 8), list_b = scratchSlot(plan, s.count * 8);
   const int partial = scratchSlot(plan, static_cast<size_t>(s.pre * pieces * 2 * s.post) * (wide ? 8 : 4));
 
   const std::string ot = storageTypeOf(s.out_dtype), bt = storageTypeOf(s.base_dtype), vt = ctypeOf(s.dtype);
@@ -551,7 +546,7 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
     l.grid[0] = static_cast<uint32_t>(8 + fillers);
     l.block[0] = 512;
     l.label = name + " order";
-    for (int slot : {s.index_slot, key_a, pos_a, key_b, pos_b, s.out_slot}) l.args.push_back(slotArg(slot));
+    for (int slot : {s.index_slot, list_a, list_b, s.out_slot}) l.args.push_back(slotArg(slot));
     if (s.base_slot >= 0) l.args.push_back(slotArg(s.base_slot));
     plan.launches.push_back(l);
   }
@@ -565,7 +560,7 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
     define(o, "PIECES", num(pieces) + "ll");
     define(o, "AHEAD", num(ahead));
     o << kSumHead << "extern \"C\" __global__ void __launch_bounds__(" << threads << ") " << name << kernel
-      << "(const unsigned int* __restrict__ keys, const unsigned int* __restrict__ places, " << vt << "* __restrict__ partial, " << ot
+      << "(const uint2* __restrict__ list, " << vt << "* __restrict__ partial, " << ot
       << "* __restrict__ out BASE_PARAM" << more << ") {\n";
   };
   auto sumLaunch = [&](int kernel, const char* what, int threads, int64_t blocks) {
@@ -576,7 +571,7 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
     l.grid[2] = static_cast<uint32_t>(s.pre);
     l.block[0] = static_cast<uint32_t>(threads);
     l.label = name + what;
-    for (int slot : {key_a, pos_a, partial, s.out_slot}) l.args.push_back(slotArg(slot));
+    for (int slot : {list_a, partial, s.out_slot}) l.args.push_back(slotArg(slot));
     if (s.base_slot >= 0) l.args.push_back(slotArg(s.base_slot));
     return l;
   };
@@ -610,7 +605,7 @@ void emitScatterAdd(const ScatterOp& s, const std::string& name, Plan& plan, con
     if (join_blocks > 65535) throw PlanError("scatter_add rows are too long");
     std::ostringstream o;
     sumHead(o, "_join", "", join_threads, join_vec, 1, 16);
-    o << "  (void)places;\n" << kJoinBody;
+    o << kJoinBody;
     plan.launches.push_back(sumLaunch(addKernel(plan, name + "_join", "scatter_add", o.str()), " join", join_threads, join_blocks));
   }
 }
