@@ -2,6 +2,7 @@
 // the log-probabilities of given tokens with their gradient.  The lookup itself is no kernel of its own:
 // a gather is an indirect row offset in whatever row kernel consumes it (emit_row.cpp).
 #include <algorithm>
+#include <iomanip>
 #include <sstream>
 
 #include "plan.hpp"
@@ -622,11 +623,10 @@ namespace {
 // one fused step and one ex2.approx per element.  c is the same for every element that is summed with it
 // or divided by the sum, so its rounding cancels, and the fused step rounds at the size of its result: rows whose
 // logits are all far from zero lose nothing.  References are combined as 2^(c1 - c2), for the same
-// reason.  A reference of 1e38 or more would overflow c: such rows (logits at the type's lowest value)
-// subtract first.  A thread moves its reference only when a logit exceeds it by more than 40: e^40 times
+// reason.  A reference of 1e34 or more might overflow c: such rows (logits at the type's lowest value)
+// subtract first.  Where the logits are others times a number, the number goes into the constant (L2E below).  A thread moves its reference only when a logit exceeds it by more than 40: e^40 times
 // any number of terms is far from the end of f32, and the sums then rarely need rescaling.
 const char* kTokenCommon = R"CUDA(
-#define L2E 1.4426950408889634f
 #define LN2 0.6931471805599453f
 #define NEG_INF __uint_as_float(0xff800000u)
 #if IN_BITS == 32
@@ -675,7 +675,7 @@ __device__ __forceinline__ float largest(unsigned int packed) {
 // whether c would overflow (f16 logits cannot get there; an infinite one gives NaN either way)
 __device__ __forceinline__ bool huge_ref(float m) {
 #if IN_BITS == 32 || IN_BF16
-  return fabsf(m) >= 1e38f && m != NEG_INF;
+  return fabsf(m) >= 1e34f && m != NEG_INF;
 #else
   return false;
 #endif
@@ -718,7 +718,7 @@ struct Sum {
     if (t > limit) {
       s = moved(s, m, t);
       m = t;
-      limit = t + 40.0f;
+      limit = t + 40.0f / SCALE;
     }
     if (huge_ref(m)) add<true>(raw);
     else add<false>(raw);
@@ -753,7 +753,7 @@ struct Sum {
   }
 };
 __device__ __forceinline__ float log_prob_at(float x, float m, float total) {
-  const float d = huge_ref(m) ? x - m : __fmaf_rn(x, L2E, minus_c(m)) * LN2;
+  const float d = huge_ref(m) ? (x - m) * SCALE : __fmaf_rn(x, L2E, minus_c(m)) * LN2;
   return d - logf(total);
 }
 
@@ -779,7 +779,7 @@ struct Slope {
   long long at;
   int vector;
   __device__ __forceinline__ Slope(float m_, float total, float slope, bool known, long long tok, float x_, int lead)
-      : m(m_), minus(minus_c(m_)), g(known ? slope : 0.0f), x(x_), at(tok), vector(known ? (int)((tok + lead) / E) : -1) {
+      : m(m_), minus(minus_c(m_)), g(known ? slope * GRAD_SCALE : 0.0f), x(x_), at(tok), vector(known ? (int)((tok + lead) / E) : -1) {
     k = -g / total;
   }
   // rows that take the slow way: those the loss does not depend on are zero whatever their logits hold
@@ -1285,6 +1285,13 @@ void emitTokenLogProb(const TokenOp& op, const std::string& name, Plan& plan, co
   define(o, "XT", storageTypeOf(op.logits_dtype));
   define(o, "TT", storageTypeOf(op.token_dtype));
   define(o, "GT", storageTypeOf(op.grad_dtype));
+  std::ostringstream l2e, scale, grad_scale;
+  l2e << std::scientific << std::setprecision(16) << 1.4426950408889634 * static_cast<double>(op.scale) << "f";
+  scale << std::scientific << std::setprecision(9) << op.scale << "f";
+  grad_scale << std::scientific << std::setprecision(9) << op.grad_scale << "f";
+  define(o, "L2E", l2e.str());
+  define(o, "SCALE", scale.str());
+  define(o, "GRAD_SCALE", grad_scale.str());
   define(o, "STORE(x)", storeConv(op.grad_dtype, "x"));
   define(o, "OUT_16", op.grad_dtype == DType::f32 ? "0" : "1");
   define(o, "OUT_16_NAME", op.grad_dtype == DType::bf16 ? "\"bf16\"" : "\"f16\"");

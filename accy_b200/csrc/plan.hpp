@@ -119,6 +119,8 @@ struct TokenOp {
   int log_prob_slot = -1;         // written when >= 0
   int stats_out = -1, stats_in = -1;  // (row maximum, sum of exponentials) written / read in place of a pass
   int grad_slot = -1;             // written when >= 0
+  float scale = 1.0f;             // the log-probabilities are those of logits * scale (scale > 0)
+  float grad_scale = 1.0f;        // the gradient is written times this
   DType grad_dtype = DType::f32;
   // The slope as an expression over the row dims; node `acc` stands for the row's log-probability.
   Epilogue slope;

@@ -233,6 +233,15 @@ class Planner {
       default:
         break;
     }
+    if (op.kind == Kind::binary) {
+      // a token gradient times a number is written that way by the kernel that computes it
+      for (uint32_t a : op.operands) {
+        double factor;
+        if (!isCall(a, Call::token_log_prob_grad) || slot_of[a] >= 0 || scaledUser(a, &factor) != v) continue;
+        planTokens(a);
+        return slot_of[v];
+      }
+    }
     if (isElementwise(op.kind) && tryGemmEpilogue(v)) return slot_of[v];
     planCluster(v);
     return slot_of[v];
@@ -1171,6 +1180,31 @@ class Planner {
     return kNone;
   }
 
+  bool isCall(uint32_t v, Call c) const { return P.ops[v].kind == Kind::custom_call && P.ops[v].sub == static_cast<uint8_t>(c); }
+
+  // The product of `v` and a number, if that is all `v` is used for; kNone otherwise.
+  uint32_t scaledUser(uint32_t v, double* factor) {
+    if (v == kNone || is_output[v] || users[v].size() != 1) return kNone;
+    const Operation& op = P.ops[users[v][0]];
+    if (op.kind != Kind::binary || op.sub != static_cast<uint8_t>(Binary::mul)) return kNone;
+    const uint32_t other = op.operands[0] == v ? op.operands[1] : op.operands[0];
+    return scalarConstant(other, factor) && std::isfinite(*factor) ? op.id : kNone;
+  }
+
+  // Logits that are other logits times a number (a temperature): the other logits, and the number.  The kernels take
+  // factors from 2^-10 to 2^10 into the constant that their exponents are multiplied by anyway.
+  uint32_t unscaled(uint32_t v, float* scale) {
+    const Operation& op = P.ops[v];
+    if (slot_of[v] >= 0 || op.kind != Kind::binary || op.sub != static_cast<uint8_t>(Binary::mul)) return v;
+    for (int side = 0; side < 2; ++side) {
+      double factor;
+      if (!scalarConstant(op.operands[side], &factor) || !(factor >= 1.0 / 1024 && factor <= 1024)) continue;
+      *scale = static_cast<float>(factor);
+      return op.operands[1 - side];
+    }
+    return v;
+  }
+
   // one value under one or two names (kNone is no value's)
   bool sameValue(uint32_t a, uint32_t b) const { return a == b || (a != kNone && b != kNone && same_as[a] == same_as[b]); }
 
@@ -1228,14 +1262,18 @@ class Planner {
     const bool is_grad = static_cast<Call>(P.ops[v].sub) == Call::token_log_prob_grad;
     uint32_t forward = is_grad ? partnerOf(v, Call::token_log_prob) : v;
     uint32_t grad = is_grad ? v : partnerOf(v, Call::token_log_prob_grad);
-    auto open = [&](uint32_t x) { return x != kNone && slot_of[x] < 0 && !produced.count(x); };
+    double grad_factor = 1.0;
+    const uint32_t product = scaledUser(grad, &grad_factor);   // written in the gradient's place
+    auto open = [&](uint32_t x) {
+      return x != kNone && slot_of[x] < 0 && !produced.count(x) && (x != grad || product == kNone || slot_of[product] < 0);
+    };
     TokenOp t;
     const Operation& any = P.ops[v];
     const Type &lt = P.typeOf(any.operands[0]), &kt = P.typeOf(any.operands[1]);
     t.vocab = lt.dims.back().extent;
     t.rows = static_cast<int64_t>(kt.elementCount());
     for (const Dim& d : kt.dims) t.row_extents.push_back(d.extent);
-    t.logits_slot = materialize(any.operands[0]);
+    t.logits_slot = materialize(unscaled(any.operands[0], &t.scale));
     t.token_slot = materialize(any.operands[1]);
     t.logits_dtype = plan.slots[t.logits_slot].storage;
     t.token_dtype = plan.slots[t.token_slot].storage;
@@ -1245,7 +1283,7 @@ class Planner {
       // the slope needs log-probabilities of other rows: they come first, in a kernel of their own,
       // which leaves its rows' maxima and sums for this one
       materializeFolds(any.operands[2]);
-      if (slot_of[v] >= 0) return;
+      if (!open(v)) return;
       forward = kNone;
       t.slope = Epilogue{};
       if (!slopeOf(any.operands[2], kNone, &t.slope)) {
@@ -1270,12 +1308,18 @@ class Planner {
       forward = kNone;
     }
     if (grad != kNone) {
+      if (product != kNone) {
+        grad = product;
+        t.grad_scale = static_cast<float>(grad_factor);
+      }
       t.grad_slot = destinationSlot(grad);
       t.grad_dtype = plan.slots[t.grad_slot].storage;
     }
     const std::string name = nextName("tokens");
     summary << "token log-probabilities: " << name << " rows=" << t.rows << " vocab=" << t.vocab << " logits=" << dtypeName(t.logits_dtype)
-            << (forward != kNone ? " value" : "") << (grad != kNone ? " gradient" : "") << (t.stats_in >= 0 ? " from kept sums" : "") << "\n";
+            << (forward != kNone ? " value" : "") << (grad != kNone ? " gradient" : "") << (t.stats_in >= 0 ? " from kept sums" : "");
+    if (t.scale != 1.0f || t.grad_scale != 1.0f) summary << " scale=" << t.scale << "," << t.grad_scale;
+    summary << "\n";
     emitTokenLogProb(t, name, plan, ov);
     plan.work.pairs += static_cast<double>(t.rows) * static_cast<double>(t.vocab);
     if (forward != kNone) {

@@ -403,6 +403,27 @@ def test_a_slope_over_whole_sequences_takes_the_kept_sums(cpu_session):
     assert len(calls) == 2 and calls[0].endswith("value") and calls[1].endswith("gradient from kept sums"), lines
 
 
+def tempered(factor, dtype="bf16"):
+    def body(b, a):
+        return nn.cross_entropy(a[0].mul(b.scalar(dtype, factor)), a[1], "vocab")
+    return body
+
+
+def test_a_temperature_joins_the_kernel(cpu_session):
+    # beyond the factors the kernel takes the product is a kernel of its own; an infinite one is not taken into the gradient either
+    for factor, joins, kernels in ((0.5, True, 3), (1024.0, True, 3), (2.0 ** -11, False, 4), (-1.0, False, 4), (float("inf"), False, 5)):
+        lines = plan_lines(cpu_session, T.define("t", [LOGITS, IDS], tempered(factor)).value_and_grad([0]))
+        calls = [x for x in lines if x.startswith("token")]
+        assert len(calls) == 1 and "value gradient" in calls[0], lines
+        assert ("scale=%g,%g" % (factor, factor) in calls[0]) == joins and len(lines) == kernels, lines
+    # a gradient that something else needs as well is written as it is
+    def both(b, a):
+        y = a[0].mul(b.scalar("bf16", 0.5))
+        return y.token_log_prob(a[1], "vocab").sum(["batch", "seq"]).add(y.token_log_prob(a[2], "vocab").sum(["batch", "seq"]))
+    calls = [x for x in plan_lines(cpu_session, T.define("t", [LOGITS, IDS, IDS], both).value_and_grad([0])) if x.startswith("token")]
+    assert len(calls) == 2 and all(x.endswith("scale=0.5,1") for x in calls), calls
+
+
 def test_a_lookup_joins_the_kernel_that_uses_it(cpu_session):
     def norm(b, a):
         x = nn.embedding(a[0], a[1], "vocab", scale=3.0)
@@ -614,6 +635,44 @@ def test_rows_of_infinities_nans_and_lowest_values(gpu_session, dtype, vocab, co
     g.reshape(copies, 9)[:, [0, 4, 5]] = 0
     got = run(gpu_session, program, [data, tok, g])[0]
     assert np.all(got.reshape(copies, 9, vocab)[:, [0, 4, 5, 8]] == 0) and np.all(np.isfinite(got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("factor", [0.5, 3.0, -1.0, 2.0 ** -11, 0.0])
+@pytest.mark.parametrize("dtype,rows,vocab", [("f32", 5, 1003), ("bf16", 300, 40000), ("f16", 2, 70001)])
+def test_logits_times_a_number(gpu_session, dtype, rows, vocab, factor):
+    x, tok = logits_and_tokens(dtype, (rows,), vocab, rows)
+    program = T.define("t", [T.spec(dtype, n=rows, vocab=vocab), T.spec("i32", n=rows)], tempered(factor, dtype)).value_and_grad([0])
+    value, grad = run(gpu_session, program, [x, tok])
+    y = factor * exactly(dtype, x)
+    want, p, hot, known = log_prob_of(y, tok)
+    n = max(known.sum(), 1)
+    step = p_error(y) + 2 * U["f32"] * (1 + spread_of(y))   # the product is rounded, or the constant that takes its place
+    close(value.reshape(()), -want.sum() / n, step + (rows + 8) * U["f32"] * np.abs(want).sum() / n)
+    exact = factor * (p - hot) * known[:, None] / n
+    close(grad, exact, abs(factor) / n * known[:, None] * (p + hot) * (step + 8 * U["f32"]) + U[dtype] * np.abs(exact) + TINY[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["gather", "scatter_add", "log_prob"])
+def test_batched_and_forward_mode_programs_on_the_device(gpu_session, op):
+    """vmap with both operands mapped, and jvp, against the oracle's f64 evaluation of the same derived programs: short f32
+    sums, 40 roundings of the largest magnitude at most."""
+    rng = np.random.default_rng(2)
+    v, n, d, size = 70, 48, 48, 5
+
+    def body(b, a):
+        if op == "gather":
+            return a[0].gather(a[1], "v")
+        if op == "scatter_add":
+            return a[0].scatter_add(a[1], a[0].gather(a[1], "v").mul(b.scalar("f32", 2.0)), "v")
+        return a[0].token_log_prob(a[1].rename("n", "d"), "v")
+    program = T.define("one", [T.spec("f32", v=v, d=d), T.spec("i32", n=n)], body)
+    x, idx = rng.standard_normal((size, v, d)).astype(np.float32), rng.integers(-2, v + 2, (size, n)).astype(np.int32)
+    for derived, inputs in ((program.vmap(size, [0, 0]), [x, idx]), (program.jvp([0]), [x[0], idx[0], x[1]]),
+                            (program.jvp([0]).vmap(size, [0, 0, None]), [x, idx, x[1]])):
+        for got, want in zip(run(gpu_session, derived, inputs), oracle.run(derived.wire, inputs, mode="f64")):
+            close(got, want, 40 * U["f32"] * (np.abs(want) + np.abs(want).max()) + p_error(x.astype(np.float64)) * np.abs(want).max())
 
 
 @pytest.mark.gpu
