@@ -96,6 +96,8 @@ struct accy_b200_session {
   CUstream_t stream = nullptr;
   int sm_count = 148;
   bool time_launches = false;      // accy_b200_session_time_launches
+  std::vector<uint64_t> argument_values;   // of the launch being issued; kept, so that a launch allocates nothing
+  std::vector<void*> argument_pointers;
   CUdeviceptr_t status_word = 0;  // device int the tcgen05 kernels set when a bounded wait gives up
 
   void observe(const char* phase, uint64_t begin_ns) {
@@ -446,8 +448,10 @@ struct accy_b200_session {
     }
     for (size_t li = 0; li < e.plan.launches.size(); ++li) {
       const Launch& l = e.plan.launches[li];
-      std::vector<uint64_t> values(l.args.size());
-      std::vector<void*> ptrs(l.args.size());
+      std::vector<uint64_t>& values = argument_values;
+      std::vector<void*>& ptrs = argument_pointers;
+      values.resize(l.args.size());
+      ptrs.resize(l.args.size());
       for (size_t a = 0; a < l.args.size(); ++a) {
         const KernelArg& arg = l.args[a];
         if (arg.tensor_map) {

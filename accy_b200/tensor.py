@@ -527,6 +527,18 @@ def _buffer_address(buf, writable):
     raise SessionError(4, "unsupported buffer type %r" % type(buf))
 
 
+_invoke_device = lib.accy_b200_session_invoke_device
+_address_arrays = {}   # array type by length: looking one up takes a tenth of what ctypes takes to make it
+
+
+def _addresses(pointers):
+    count = len(pointers)
+    kind = _address_arrays.get(count)
+    if kind is None:
+        kind = _address_arrays[count] = ctypes.c_uint64 * max(1, count)
+    return kind(*pointers)
+
+
 class Session:
     """tensor.session.Session (src/tensor/session/session.zig:88-246) on a B200."""
 
@@ -602,10 +614,12 @@ class Session:
         del keep
 
     def invoke_device(self, compiled, input_ptrs, output_ptrs, stream=None):
-        ins = (ctypes.c_uint64 * max(1, len(input_ptrs)))(*input_ptrs)
-        outs = (ctypes.c_uint64 * max(1, len(output_ptrs)))(*output_ptrs)
-        self._check(lib.accy_b200_session_invoke_device(self._h, compiled.handle, ins, len(input_ptrs), outs,
-                                                        len(output_ptrs), ctypes.c_void_p(stream or 0)))
+        """Launches on device buffers, given as addresses, without copies and without waiting.  `stream` is a
+        CUstream handle (1 is the legacy default stream, torch's `cuda_stream` 0); None is the session's own."""
+        status = _invoke_device(self._h, compiled.handle, _addresses(input_ptrs), len(input_ptrs), _addresses(output_ptrs),
+                                len(output_ptrs), stream or None)
+        if status:
+            self._check(status)
 
     def synchronize(self, stream=None):
         self._check(lib.accy_b200_session_synchronize(self._h, ctypes.c_void_p(stream or 0)))
