@@ -44,8 +44,8 @@ def _counted(logits, tokens, axis, mask):
         raise TensorError("NonIntegerDType")
     zero = b.scalar("f32", 0.0)
     weight = b.scalar("f32", 1.0) if mask is None else mask
-    if extent - 1 < _LARGEST[dtype]:
-        weight = tokens.compare("le", b.scalar(dtype, extent - 1)).select(weight, zero)
+    if extent <= _LARGEST[dtype]:   # otherwise no number of the type is past the end
+        weight = tokens.compare("lt", b.scalar(dtype, extent)).select(weight, zero)
     weight = tokens.compare("ge", b.scalar(dtype, 0)).select(weight, zero)
     return weight, weight.compare("ne", zero)
 

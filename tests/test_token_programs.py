@@ -262,6 +262,29 @@ def test_gradients_match_differences(name):
     differences(program, inputs, 0, grad)
 
 
+def test_gradients_with_respect_to_the_other_inputs_of_the_policy_loss():
+    """The advantage is one number per sequence, stretched over its tokens: its gradient sums over them."""
+    program, inputs = policy_program(), small_inputs()
+    grads = oracle.run(program.grad([2, 3, 4]).wire, inputs, mode="f64")
+    for index, grad in zip((2, 3, 4), grads):
+        differences(program, inputs, index, grad)
+    assert grads[0][0, 2] == 0 and grads[1][0, 2] == 0 and grads[0][1, 1] == 0   # masked, and a token outside
+
+
+def test_token_types_and_vocabularies_at_their_ends():
+    """Losses record for every token type, also where the vocabulary is as large as the type or empty."""
+    for dtype, extent in (("u8", 256), ("u8", 255), ("i8", 128), ("i8", 5), ("u8", 0), ("u64", 3)):
+        specs = [T.spec("f32", n=4, v=extent), T.spec(dtype, n=4)]
+        program = T.define("ce", specs, lambda b, a: nn.cross_entropy(a[0], a[1], "v"))
+        tok = np.array([0, 3, 127, 4], NP[dtype])
+        x = np.random.default_rng(1).standard_normal((4, extent)).astype(np.float32)
+        want = 0.0
+        if extent:
+            log_p, _, _, known = log_prob_of(x.astype(np.float64), tok)
+            want = -log_p.sum() / max(known.sum(), 1)
+            assert abs(float(oracle.run(program.wire, [x, tok], mode="f64")[0].reshape(-1)[0]) - want) < 1e-12
+
+
 def test_gradient_of_scatter_add_and_repeated_lookups():
     def body(b, a):
         base, idx, up, weight = a
@@ -673,6 +696,16 @@ def test_batched_and_forward_mode_programs_on_the_device(gpu_session, op):
                             (program.jvp([0]).vmap(size, [0, 0, None]), [x, idx, x[1]])):
         for got, want in zip(run(gpu_session, derived, inputs), oracle.run(derived.wire, inputs, mode="f64")):
             close(got, want, 40 * U["f32"] * (np.abs(want) + np.abs(want).max()) + p_error(x.astype(np.float64)) * np.abs(want).max())
+
+
+@pytest.mark.gpu
+def test_policy_gradients_of_every_input_on_the_device(gpu_session):
+    inputs = policy_case("f32", 3, 70, 1003, 5)
+    program = policy_program("f32", "i32", 3, 70, 1003).value_and_grad([0, 2, 3, 4])
+    for got, want in zip(run(gpu_session, program, inputs), oracle.run(program.wire, inputs, mode="f64")):
+        # ratios off by the error of a log-probability, then f32 sums of at most 210 terms
+        scale = np.abs(want).max()
+        close(got.reshape(want.shape), want, (4 * p_error(exactly("f32", inputs[0])) + 300 * U["f32"]) * (np.abs(want) + scale))
 
 
 @pytest.mark.gpu
