@@ -1315,13 +1315,16 @@ void emitTokenLogProb(const TokenOp& op, const std::string& name, Plan& plan, co
   define(o, "LOG_PROB_OUT", op.log_prob_slot >= 0 ? "1" : "0");
   define(o, "GRADIENT", gradient ? "1" : "0");
   define(o, "LEAF_PARAMS", gradient ? slope.params() : "");
-  // One CTA of 24 warps per SM with a ring of 216 KB for rows of which two such rings hold too little, two CTAs of 16
-  // warps with 96 KB each for shorter ones, whose own latencies then overlap (bf16 4096 x 50001: 174 us with two, 193 us
-  // with one; f32 8192 x 32768: 401 and 348 us; bf16 8192 x 131072: 948 and 711 us).  16-bit logits ask for twice the
-  // arithmetic per byte, so two CTAs serve them up to longer rows.
+  // One CTA of up to 27 warps per SM with a ring of 216 KB for rows of which two smaller rings hold too little, two CTAs of up
+  // to 16 warps with 112 KB each for shorter ones, whose own latencies then overlap (bf16 4096 x 50001: 176 us with two, 188
+  // with one; f32 8192 x 32768: 377 and 340 us; bf16 8192 x 131072: 797 and 709 us).  16-bit logits ask for twice the
+  // arithmetic per byte, so two CTAs serve them up to longer rows.  Two vectors per thread make a chunk, and a
+  // row is cut into equal ones: a last chunk of a few vectors would take as long as a whole one (bf16 4096 x 50001 in seven
+  // equal chunks 172 us).
   const bool wide_ring = row_bytes >= (in_size == 4 ? 112 : 160) * 1024;
-  const int64_t slots = wide_ring ? 9 : 6, chunk = wide_ring ? 1536 : 1024, consumers = wide_ring ? 768 : 512;
-  const int64_t ctas = wide_ring ? 1 : 2, hold = wide_ring ? 7 : 5;
+  const int64_t ctas = wide_ring ? 1 : 2, ring_bytes = (wide_ring ? 216 : 112) * 1024, most_chunk = wide_ring ? 1728 : 1024;
+  const int64_t chunk = ceilDiv(ceilDiv(vectors, ceilDiv(vectors, most_chunk)), 64) * 64, consumers = chunk / 2;
+  const int64_t slots = ring_bytes / (chunk * 16), hold = slots - 1;
   // A gradient of which more than half is computed from logits read again is written past L2, where it would take
   // their place (f32 2048 x 150000: 522 and 481 us; bf16 8192 x 32768, nothing read again: 182 and 188 us).
   define(o, "WRITE(p, v)", stream && row_bytes > 2 * hold * chunk * 16 ? "__stcs(p, v)" : "*(p) = (v)");
