@@ -618,7 +618,7 @@ namespace {
 
 // The arithmetic.  With c = fl(m log2 e) for a reference m near the row's maximum,
 //
-//   e[v] = 2^(x[v] log2 e - c)    log p = ln 2 (x[token] log2 e - c) - ln(sum e)    p[v] = e[v] / sum e
+//   e[v] = 2^(x[v] log2 e - c)    log p = (x[token] - m) - (ln(sum e) - ln 2 (m log2 e - c))    p[v] = e[v] / sum e
 //
 // one fused step and one ex2.approx per element.  c is the same for every element that is summed with it
 // or divided by the sum, so its rounding cancels, and the fused step rounds at the size of its result: rows whose
@@ -752,9 +752,11 @@ struct Sum {
     for (int off = W / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off, W);
   }
 };
+// (x - m) - log(sum of e^(x - m)): the sum is relative to c instead of m log2 e, which is off by a known residue.  The
+// difference is taken before anything is rounded at the size of x.
 __device__ __forceinline__ float log_prob_at(float x, float m, float total) {
-  const float d = huge_ref(m) ? (x - m) * SCALE : __fmaf_rn(x, L2E, minus_c(m)) * LN2;
-  return d - logf(total);
+  const float residue = huge_ref(m) ? 0.0f : __fmaf_rn(m, L2E, minus_c(m));
+  return (x - m) * SCALE - (logf(total) - residue * LN2);
 }
 
 #if GRADIENT
