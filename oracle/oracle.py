@@ -465,18 +465,18 @@ class Evaluator:
             elif k == "dot_general":
                 vals[op.id] = self._round(op.dtype, self._dot(vals[op.operands[0]], vals[op.operands[1]], op.lists))
             elif k == "gather":
-                x, idx = vals[op.operands[0]], vals[op.operands[1]]
+                x, idx = (vals[i].reshape(_shape(ops[i].dims)) for i in op.operands)   # rank-0 values are held with one axis
                 vals[op.id] = _lookup(x, idx, op.axis)
             elif k == "scatter_add":
-                base, idx, up = (vals[i] for i in op.operands)
+                base, idx, up = (vals[i].reshape(_shape(ops[i].dims)) for i in op.operands)
                 vals[op.id] = self._round(op.dtype, _scatter_add(base, idx, up, op.axis))
             elif k == "custom_call":
-                x, tok = vals[op.operands[0]], vals[op.operands[1]]
+                x, tok = (vals[i].reshape(_shape(ops[i].dims)) for i in op.operands[:2])
                 log_prob, p, hot = _token_log_prob(x, tok, op.axis)
                 if op.sub.endswith("prob"):
                     vals[op.id] = log_prob
                 else:
-                    g = np.expand_dims(vals[op.operands[2]], op.axis)
+                    g = np.expand_dims(vals[op.operands[2]].reshape(_shape(op.dims[:op.axis] + op.dims[op.axis + 1:])), op.axis)
                     with np.errstate(all="ignore"):
                         grad = np.where((g == 0) | (hot.sum(op.axis, keepdims=True) == 0), 0, (hot - p) * g).astype(x.dtype)
                     vals[op.id] = self._round(op.dtype, grad)

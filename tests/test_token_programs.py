@@ -827,6 +827,78 @@ def test_lookup_head_loss_and_both_gradients_together(gpu_session, dtype, sizes)
     close(got[0].reshape(()), want[0].reshape(()), (4 * U[dtype] + 1e-5) * abs(float(want[0].reshape(-1)[0])))
 
 
+def random_token_program(seed):
+    """A lookup in a table of one to three axes by numbers of none to two, what follows it elementwise, folds of it, a scatter back
+    into the table, a second lookup and the log-probability of tokens along some axis of it, with a gradient."""
+    rng = np.random.default_rng(900 + seed)
+    pick = lambda *xs: xs[rng.integers(len(xs))]  # noqa: E731
+    extent = lambda: int(pick(1, 2, 3, 5, 8, 16, 33, 64, 130))  # noqa: E731
+    table = {"t%d" % i: extent() for i in range(rng.integers(1, 4))}
+    axis = pick(*table)
+    ids = {"i%d" % i: extent() for i in range(rng.integers(0, 3))}
+    looked = [n for n in list(table)[:list(table).index(axis)]] + list(ids) + [n for n in list(table)[list(table).index(axis) + 1:]]
+    dims = {**table, **ids}
+    specs = [T.spec("f32", **table), T.spec(pick("i32", "i64", "i16"), **ids)]
+    bias = {n: dims[n] for n in looked if rng.random() < 0.5}
+    specs.append(T.spec("f32", **dict(reversed(list(bias.items())))))
+    vocab = pick(*looked) if looked else None
+    if vocab:
+        specs.append(T.spec("i32", **{n: dims[n] for n in reversed(looked) if n != vocab}))
+    transposed, fold = rng.random() < 0.4, pick(*looked) if looked else None
+
+    def body(b, a):
+        source = a[0].mul(b.scalar("f32", 1.5)) if transposed else a[0]
+        x = source.gather(a[1], axis)
+        y = x.mul(x).sub(a[2])
+        outs = [y, a[0].scatter_add(a[1], y.mul(b.scalar("f32", 0.5)), axis)]
+        if fold:
+            outs += [y.sum(fold), x.max(fold)]
+        if vocab:
+            outs.append(y.token_log_prob(a[3], vocab))
+        return outs
+
+    def loss(b, a):
+        x = a[0].gather(a[1], axis)
+        y = x.mul(a[2]).add(x)
+        total = y.sum(list(looked)) if looked else y
+        if vocab:
+            log_prob = y.token_log_prob(a[3], vocab)
+            names = [n for n, _ in log_prob.ty.dims]
+            total = total.add(log_prob.sum(names) if names else log_prob)
+        return total
+    inputs = []
+    for s in specs:
+        shape = tuple(e for _, e in s.dims)
+        if s.dtype == "f32":
+            inputs.append(rng.standard_normal(shape).astype(np.float32))
+        else:
+            top = table[axis] if len(inputs) == 1 else dims[vocab]
+            inputs.append(np.asarray(rng.integers(-1, top + 1, shape)).astype(NP[s.dtype]))
+    return specs, body, loss, inputs
+
+
+@pytest.mark.parametrize("seed", range(32))
+def test_random_token_programs_plan(cpu_session, seed):
+    specs, body, loss, _ = random_token_program(seed)
+    for program in (T.define("r", specs, body), T.define("l", specs, loss).value_and_grad([0, 2])):
+        compiled = cpu_session.compile(program)
+        cpu_session.release(compiled)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(32))
+def test_random_token_programs_match_the_oracle(gpu_session, seed):
+    """Values of size about one, f32 sums of at most 130 * 130 of them and exponentials of them: 1e-5 of the largest
+    magnitude (sums of n terms of both signs: n * 2^-24 * mean magnitude at most, reached by no fold in trees).  The gradient
+    at a token is g - g * p: four roundings of g, which is 1 here, also where p is 1 and nothing else is left (a vocabulary of
+    one), times the derivative 1 + bias of y, at most 6 in these inputs: 6 * 4 * 2^-24 < 2e-6."""
+    specs, body, loss, inputs = random_token_program(seed)
+    for program in (T.define("r", specs, body), T.define("l", specs, loss).value_and_grad([0, 2])):
+        for got, want in zip(run(gpu_session, program, inputs), oracle.run(program.wire, inputs, mode="f64")):
+            want = np.asarray(want).reshape(got.shape)
+            close(got, want, 1e-5 * (np.abs(want) + (np.abs(want).max() if want.size else 0)) + 2e-6)
+
+
 def torch_buffers(program, inputs):
     import torch
     given = [torch.from_numpy(np.ascontiguousarray(x.view(np.int16) if x.dtype == np.uint16 else x)).cuda() for x in inputs]
