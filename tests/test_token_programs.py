@@ -979,6 +979,66 @@ def test_captured_replayed_and_on_other_streams(which):
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Buffers of more than 2^32 bytes and 2^31 elements: the rows at both ends of a table, of its gradient, and of a batch of logits."""
+    import torch
+    free = torch.cuda.mem_get_info()[0]
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    vocab, dim = 600011, 4096
+    table = torch.zeros(vocab, dim, dtype=torch.bfloat16, device="cuda")
+    ids = torch.tensor([0, vocab - 1, 524287, 524288, vocab - 1, -1, vocab], dtype=torch.int64, device="cuda")
+    known = ids.clamp(0, vocab - 1)
+    table[known] = torch.randn(7, dim, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    rows = torch.full((7, dim), 3.0, dtype=torch.bfloat16, device="cuda")
+    program = T.define("e", [T.spec("bf16", v=vocab, d=dim), T.spec("i64", n=7)], lambda b, a: nn.embedding(a[0], a[1], "v", scale=2.0))
+    cuda = T.Cuda(program, device=0)
+    cuda.launch_device([table.data_ptr(), ids.data_ptr()], [rows.data_ptr()], 1)
+    torch.cuda.synchronize()
+    want = table[known] * 2.0
+    want[5:] = 0
+    assert torch.equal(rows, want)
+    cuda.deinit()
+    # the gradient over the same table: row sums at both ends, zeros elsewhere
+    up = torch.randn(7, dim, device="cuda").bfloat16()
+    out = table
+    out.fill_(9.0)
+    program = T.define("s", [T.spec("i64", n=7), T.spec("bf16", n=7, d=dim)], lambda b, a: nn.embedding_grad(a[0], a[1], "v", vocab))
+    cuda = T.Cuda(program, device=0)
+    cuda.launch_device([ids.data_ptr(), up.data_ptr()], [out.data_ptr()], 1)
+    torch.cuda.synchronize()
+    expected = {0: up[0], vocab - 1: (up[1].float() + up[4].float()).bfloat16(), 524287: up[2], 524288: up[3]}
+    for row, values in expected.items():
+        assert torch.equal(out[row], values)
+    out[list(expected)] = 0
+    assert not bool(out.any())
+    cuda.deinit()
+    del table, out
+    # logits of 36007 x 60001: the last rows start beyond 2^32 bytes
+    n, v = 36007, 60001
+    logits = torch.zeros(n, v, dtype=torch.bfloat16, device="cuda")
+    tok = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    at = [0, 35789, 35794, n - 1]     # 35794 * 60001 is the first element past 2^31
+    logits[at] = torch.randn(4, v, device="cuda").bfloat16()
+    tok[at] = torch.tensor([5, 0, 60000, 31], dtype=torch.int32, device="cuda")
+    loss, grad = torch.zeros((), device="cuda"), torch.full((n, v), 7.0, dtype=torch.bfloat16, device="cuda")
+    program = T.define("c", [T.spec("bf16", n=n, v=v), T.spec("i32", n=n)], lambda b, a: nn.cross_entropy(a[0], a[1], "v")).value_and_grad([0])
+    cuda = T.Cuda(program, device=0)
+    torch.cuda.synchronize()
+    cuda.launch_device([logits.data_ptr(), tok.data_ptr()], [loss.data_ptr(), grad.data_ptr()], 1)
+    torch.cuda.synchronize()
+    x, t = logits[at].double().cpu().numpy(), tok[at].cpu().numpy()
+    log_p, p, hot, _ = log_prob_of(x, t)
+    close(float(loss), -log_p.sum() / 4, p_error(x) + 8 * U["f32"] * 12)
+    exact = (p - hot) / 4
+    close(grad[at].double().cpu().numpy(), exact, (p_error(x) + 8 * U["f32"]) * (p + hot) / 4 + U["bf16"] * np.abs(exact) + TINY["bf16"])
+    grad[at] = 0
+    assert not bool(grad.any())
+    cuda.deinit()
+
+
+@pytest.mark.gpu
 def test_host_invoke_in_chunks_equals_one_shot():
     """A large lookup and a large scoring call stream through the device in chunks; the table's gradient does not."""
     rng = np.random.default_rng(6)
