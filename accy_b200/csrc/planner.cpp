@@ -1168,7 +1168,14 @@ class Planner {
   // log-probabilities of tokens, and their gradient
   // ---------------------------------------------------------------------------------------
   static constexpr uint32_t kNone = 0xffffffffu;
-  std::map<uint32_t, int> stats_of;   // log-probability op -> slot with its rows' maxima and sums
+  // Rows' maxima and sums that a log-probability's kernel has left, with the logits and the factor they were made from:
+  // a product may get a buffer of its own after one call was planned and before the next, and sums of
+  // x times a factor are no sums of the product.
+  struct KeptSums {
+    int slot = -1, logits_slot = -1;
+    float scale = 1.0f;
+  };
+  std::map<uint32_t, KeptSums> stats_of;   // by log-probability op
 
   // the call of the given kind on the same logits and tokens as `v` that something needs
   uint32_t partnerOf(uint32_t v, Call want) {
@@ -1275,7 +1282,6 @@ class Planner {
     for (const Dim& d : kt.dims) t.row_extents.push_back(d.extent);
     t.logits_slot = materialize(unscaled(any.operands[0], &t.scale));
     t.token_slot = materialize(any.operands[1]);
-    t.logits_dtype = plan.slots[t.logits_slot].storage;
     t.token_dtype = plan.slots[t.token_slot].storage;
     const bool both = open(forward) && open(grad) && elementwiseFrom(P.ops[grad].operands[2], forward) &&
                       slopeOf(P.ops[grad].operands[2], forward, &t.slope);
@@ -1293,12 +1299,16 @@ class Planner {
       }
       const uint32_t first = partnerOf(v, Call::token_log_prob);
       auto stats = first == kNone ? stats_of.end() : stats_of.find(first);
-      if (stats != stats_of.end()) t.stats_in = stats->second;
+      if (stats != stats_of.end()) {
+        t.stats_in = stats->second.slot;
+        t.logits_slot = stats->second.logits_slot;
+        t.scale = stats->second.scale;
+      }
     }
     if (!both && !is_grad) {
       if (open(grad)) {
         t.stats_out = newSlot(Slot::Temp, static_cast<size_t>(t.rows) * 8, v, DType::f32);
-        stats_of[v] = t.stats_out;
+        stats_of[v] = KeptSums{t.stats_out, t.logits_slot, t.scale};
       }
       grad = kNone;
     }
@@ -1315,6 +1325,7 @@ class Planner {
       t.grad_slot = destinationSlot(grad);
       t.grad_dtype = plan.slots[t.grad_slot].storage;
     }
+    t.logits_dtype = plan.slots[t.logits_slot].storage;
     const std::string name = nextName("tokens");
     summary << "token log-probabilities: " << name << " rows=" << t.rows << " vocab=" << t.vocab << " logits=" << dtypeName(t.logits_dtype)
             << (forward != kNone ? " value" : "") << (grad != kNone ? " gradient" : "") << (t.stats_in >= 0 ? " from kept sums" : "");
