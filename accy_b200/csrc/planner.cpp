@@ -134,6 +134,12 @@ class Planner {
       if (want != have && plan.slots[want].bytes) copies.push_back({have, want});
     }
     for (auto& c : copies) emitCopy(c.first, c.second);
+    for (const Launch& l : plan.launches) {
+      for (const KernelArg& a : l.args) {
+        const int slot = a.tensor_map ? a.tma.slot : a.is_slot && a.slot != -2 ? a.slot : 0;
+        if (slot < 0 || slot >= static_cast<int>(plan.slots.size())) throw PlanError("internal: a kernel argument without a buffer");
+      }
+    }
     plan.summary = summary.str();
     return std::move(plan);
   }
@@ -192,7 +198,12 @@ class Planner {
 
   // Ensures v lives in a device buffer laid out row-major in its own dims; returns the slot.
   int materialize(uint32_t v) {
-    if (slot_of[v] >= 0) return slot_of[v];
+    const int slot = slot_of[v] >= 0 ? slot_of[v] : planValue(v);
+    if (slot < 0) throw PlanError(std::string("internal: a value was planned without a buffer: ") + kindName(P.ops[v].kind));
+    return slot;
+  }
+
+  int planValue(uint32_t v) {
     if (same_as[v] != v && !is_output[v] && narrow.count(v) == narrow.count(same_as[v])) {
       // the same value was (or is now) computed under an earlier name: read that buffer
       const int s = materialize(same_as[v]);
@@ -238,7 +249,7 @@ class Planner {
       for (uint32_t a : op.operands) {
         double factor;
         if (!isCall(a, Call::token_log_prob_grad) || slot_of[a] >= 0 || scaledUser(a, &factor) != v) continue;
-        planTokens(a);
+        planTokens(a, /*for_product=*/true);
         return slot_of[v];
       }
     }
@@ -1264,13 +1275,17 @@ class Planner {
     return true;
   }
 
-  void planTokens(uint32_t v) {
+  // Gives v a buffer, together with the call of the other kind on the same logits and tokens where one kernel can compute
+  // both.  A gradient whose one use is a product with a number is written as that product when the product is what was
+  // asked for, or when the gradient is only taken along; asked for itself (a region computes the product
+  // among other things) it is written as it is.
+  void planTokens(uint32_t v, bool for_product = false) {
     Depth depth(cluster_depth);
     const bool is_grad = static_cast<Call>(P.ops[v].sub) == Call::token_log_prob_grad;
     uint32_t forward = is_grad ? partnerOf(v, Call::token_log_prob) : v;
     uint32_t grad = is_grad ? v : partnerOf(v, Call::token_log_prob_grad);
     double grad_factor = 1.0;
-    const uint32_t product = scaledUser(grad, &grad_factor);   // written in the gradient's place
+    const uint32_t product = is_grad && !for_product ? kNone : scaledUser(grad, &grad_factor);   // written in the gradient's place
     auto open = [&](uint32_t x) {
       return x != kNone && slot_of[x] < 0 && !produced.count(x) && (x != grad || product == kNone || slot_of[product] < 0);
     };

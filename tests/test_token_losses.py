@@ -6,7 +6,7 @@ CPU: what the planner makes of them.  GPU: values and gradients against the orac
 import numpy as np
 import pytest
 
-from accy_b200 import tensor
+from accy_b200 import nn, tensor
 from oracle import oracle
 from test_token_programs import close, exactly, p_error, plan_lines, run, stored, U
 
@@ -70,3 +70,90 @@ def test_gradients_of_sequences_under_a_temperature(gpu_session, company, dtype,
     grad = want[1].reshape(got[1].shape)
     close(got[1], grad, 2 * step * factor * (size / (64 * n) + row) + U[dtype] * np.abs(grad))
     close(got[0].reshape(()), float(want[0].reshape(-1)[0]), 2 * step * size)
+
+
+# ---------------------------------------------------------------------------------------------
+# a gradient whose product with a number is one value among others of a region
+# ---------------------------------------------------------------------------------------------
+def scaled(b, x, factor):
+    return x.mul(b.scalar(x.ty.dtype, factor))
+
+
+def soft_capped(b, x):
+    return scaled(b, scaled(b, x, 1.0 / 32).tanh(), 32.0)
+
+
+def beside(name):
+    """(body, names of the inputs, which of them are differentiated) of a loss on scaled logits beside something else"""
+    tokens = lambda b, x, a: nn.cross_entropy(x, a["tok"], "vocab")  # noqa: E731
+    return {
+        "soft cap": (lambda b, a: tokens(b, soft_capped(b, a["x"]), a), ["x", "tok"], [0]),
+        "soft cap of a contraction": (lambda b, a: tokens(b, soft_capped(b, a["h"].contract(a["w"], "d")), a), ["h", "w", "tok"], [0, 1]),
+        "scaled and plain": (lambda b, a: tokens(b, scaled(b, a["x"], 0.5), a).add(tokens(b, a["x"], a)), ["x", "tok"], [0]),
+        "two temperatures": (lambda b, a: tokens(b, scaled(b, a["x"], 0.5), a).add(tokens(b, scaled(b, a["x"], 2.0), a)), ["x", "tok"], [0]),
+        "a bias alone": (lambda b, a: tokens(b, scaled(b, a["x"].add(a["bias"]), 0.5), a), ["x", "tok", "bias"], [2]),
+        "centred": (lambda b, a: tokens(b, scaled(b, a["x"].sub(a["x"].mean("vocab")), 0.5), a), ["x", "tok"], [0]),
+        "squares": (lambda b, a: tokens(b, scaled(b, a["x"], 0.5), a).add(scaled(b, a["x"].mul(a["x"]).sum(["n", "vocab"]), 2.0 ** -10)), ["x", "tok"], [0]),
+        "squares and a sequence": (lambda b, a: scaled(b, scaled(b, a["x"], 0.5).token_log_prob(a["tok"], "vocab").sum("n"), 1.0 / 64).tanh().add(
+            scaled(b, a["x"].mul(a["x"]).sum(["n", "vocab"]), 2.0 ** -10)), ["x", "tok"], [0]),
+        "the same twice": (lambda b, a: tokens(b, scaled(b, a["x"], 0.5), a).add(tokens(b, scaled(b, a["x"], 0.5), a)), ["x", "tok"], [0]),
+        "the same under another number": (lambda b, a: tokens(b, scaled(b, a["x"], 0.5), a).add(scaled(b, tokens(b, scaled(b, a["x"], 0.5), a), 3.0)), ["x", "tok"], [0]),
+    }[name]
+
+
+BESIDE = [(name, dtype) for name in ("soft cap", "soft cap of a contraction", "scaled and plain", "two temperatures", "a bias alone", "centred",
+                                     "squares", "squares and a sequence", "the same twice", "the same under another number")
+          for dtype in ("f32", "bf16") if dtype == "f32" or "squares" not in name]   # a sum of bf16 squares is no f32 term of a loss
+
+
+def beside_program(name, dtype, n=6, vocab=40, d=8):
+    body, names, wrt = beside(name)
+    specs = {"x": T.spec(dtype, n=n, vocab=vocab), "tok": T.spec("i32", n=n), "bias": T.spec(dtype, vocab=vocab), "h": T.spec(dtype, n=n, d=d), "w": T.spec(dtype, d=d, vocab=vocab)}
+    return T.define("beside", [specs[k] for k in names], lambda b, a: body(b, dict(zip(names, a)))), names, wrt
+
+
+@pytest.mark.parametrize("name,dtype", BESIDE)
+def test_losses_on_scaled_logits_beside_other_things_plan(cpu_session, name, dtype):
+    program, _, wrt = beside_program(name, dtype)
+    for derived in (program.value_and_grad(wrt), program.grad(wrt)):
+        assert token_calls(plan_lines(cpu_session, derived))
+
+
+def beside_magnitudes(name, wrt, inputs, n):
+    """(largest |gradient| the terms of each differentiated input can add up to, |value| its terms can), from
+    |d log p / d logit| <= 1, |tanh'| <= 1 and the numbers of the program"""
+    x = np.abs(inputs["x"]).max()
+    per_logit = {"scaled and plain": 1.5 / n, "two temperatures": 2.5 / n, "centred": 2 * 0.5 / n, "a bias alone": 0.5, "squares": 0.5 / n + 2.0 ** -9 * x,
+                 "squares and a sequence": 0.5 / 64 + 2.0 ** -9 * x, "the same twice": 1.0 / n, "the same under another number": 2.0 / n}.get(name, 1.0 / n)
+    squares = 2.0 ** -10 * (inputs["x"] ** 2).sum() if "squares" in name else 0.0
+    if name == "soft cap of a contraction":   # sum_v |d / d logit| <= 2 / n per row
+        return [2.0 / n * np.abs(inputs["w"]).max(), np.abs(inputs["h"]).max()], 1.0
+    return [per_logit] * len(wrt), 1.0 + squares
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [(6, 40, 8), (310, 5003, 64), (299, 33001, 8)])
+@pytest.mark.parametrize("name,dtype", BESIDE)
+def test_losses_on_scaled_logits_beside_other_things(gpu_session, name, dtype, sizes):
+    """Elementwise operations round at the size of their results (tanh to two roundings), sums have at most n, vocab or n * vocab
+    terms; a contraction reads the 16-bit rounding of the logits' gradient and sums f32 products."""
+    n, vocab, d = sizes
+    rng = np.random.default_rng(n)
+    program, names, wrt = beside_program(name, dtype, n, vocab, d)
+    values = {"x": stored(dtype, 2.0 * rng.standard_normal((n, vocab))), "tok": rng.integers(-1, vocab + 1, (n,)).astype(np.int32),
+              "bias": stored(dtype, rng.standard_normal(vocab)), "h": stored(dtype, rng.standard_normal((n, d))),
+              "w": stored(dtype, rng.standard_normal((d, vocab)))}
+    inputs = [values[k] for k in names]
+    derived = program.value_and_grad(wrt)
+    got, want = run(gpu_session, derived, inputs), oracle.run(derived.wire, inputs, mode="f64")
+    exact = {k: exactly(dtype, v) if k != "tok" else v for k, v in values.items()}
+    logits = exact["h"] @ exact["w"] if "contraction" in name else exact["x"] + (exact["bias"] if "bias" in name else 0)
+    top = np.abs(logits).max() * (2.0 if name == "two temperatures" else 1.0)
+    sums = (n + vocab + 64) * U["f32"]
+    # what a logit is off by moves a probability by as much, relative to it
+    step = p_error(2.0 * logits) + 16 * U["f32"] * (1 + top) + (d * U["f32"] * (np.abs(exact["h"]) @ np.abs(exact["w"])).max() if "contraction" in name else 0)
+    magnitudes, size = beside_magnitudes(name, wrt, exact, n)
+    close(got[0].reshape(()), float(want[0].reshape(-1)[0]), (2 * step + sums) * (size + np.abs(float(want[0].reshape(-1)[0]))))
+    for g, w, m in zip(got[1:], want[1:], magnitudes):
+        w = w.reshape(g.shape)
+        close(g, w, (2 * step + sums + (U[dtype] if "contraction" in name else 0)) * m + U[dtype] * np.abs(w))
