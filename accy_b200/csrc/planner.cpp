@@ -1187,6 +1187,13 @@ class Planner {
     float scale = 1.0f;
   };
   std::map<uint32_t, KeptSums> stats_of;   // by log-probability op
+  std::multiset<uint32_t> begun;           // gradients that are being planned (outer calls of planTokens)
+  struct Begun {
+    std::multiset<uint32_t>& set;
+    std::multiset<uint32_t>::iterator at;
+    Begun(std::multiset<uint32_t>& s, uint32_t v) : set(s), at(s.insert(v)) {}
+    ~Begun() { set.erase(at); }
+  };
 
   // the call of the given kind on the same logits and tokens as `v` that something needs
   uint32_t partnerOf(uint32_t v, Call want) {
@@ -1298,40 +1305,44 @@ class Planner {
     t.logits_slot = materialize(unscaled(any.operands[0], &t.scale));
     t.token_slot = materialize(any.operands[1]);
     t.token_dtype = plan.slots[t.token_slot].storage;
-    const bool both = open(forward) && open(grad) && elementwiseFrom(P.ops[grad].operands[2], forward) &&
-                      slopeOf(P.ops[grad].operands[2], forward, &t.slope);
-    if (!both && is_grad) {
-      // the slope needs log-probabilities of other rows: they come first, in a kernel of their own,
-      // which leaves its rows' maxima and sums for this one
-      materializeFolds(any.operands[2]);
-      if (!open(v)) return;
-      forward = kNone;
-      t.slope = Epilogue{};
-      if (!slopeOf(any.operands[2], kNone, &t.slope)) {
-        materialize(any.operands[2]);
+    // A value takes no gradient along whose planning has begun: what that gradient's slope needs is being planned right now.
+    const bool may_join = open(forward) && open(grad) && (is_grad || !begun.count(same_as[grad]));
+    bool both = false;
+    if (is_grad || may_join) {
+      Begun here(begun, same_as[grad]);
+      both = may_join && elementwiseFrom(P.ops[grad].operands[2], forward) && slopeOf(P.ops[grad].operands[2], forward, &t.slope);
+      if (!both && is_grad) {
+        // the slope needs log-probabilities of other rows: they come first, in a kernel of their own,
+        // which leaves its rows' maxima and sums for this one
+        materializeFolds(any.operands[2]);
+        forward = kNone;
         t.slope = Epilogue{};
-        if (!slopeOf(any.operands[2], kNone, &t.slope)) throw PlanError("internal: slope of a token gradient");
+        if (!slopeOf(any.operands[2], kNone, &t.slope)) {
+          materialize(any.operands[2]);
+          t.slope = Epilogue{};
+          if (!slopeOf(any.operands[2], kNone, &t.slope)) throw PlanError("internal: slope of a token gradient");
+        }
       }
+    }
+    // what the slope needed may have brought either call along
+    if (!open(forward)) forward = kNone;
+    const bool gradient_to_come = !is_grad && !both && open(grad);
+    if (!open(grad) || (!is_grad && !both)) grad = kNone;
+    if (forward == kNone && grad == kNone) return;
+    if (grad != kNone && forward == kNone) {
       const uint32_t first = partnerOf(v, Call::token_log_prob);
-      auto stats = first == kNone ? stats_of.end() : stats_of.find(first);
+      auto stats = first == kNone ? stats_of.end() : stats_of.find(same_as[first]);
       if (stats != stats_of.end()) {
         t.stats_in = stats->second.slot;
         t.logits_slot = stats->second.logits_slot;
         t.scale = stats->second.scale;
       }
     }
-    if (!both && !is_grad) {
-      if (open(grad)) {
-        t.stats_out = newSlot(Slot::Temp, static_cast<size_t>(t.rows) * 8, v, DType::f32);
-        stats_of[v] = KeptSums{t.stats_out, t.logits_slot, t.scale};
-      }
-      grad = kNone;
+    if (gradient_to_come) {
+      t.stats_out = newSlot(Slot::Temp, static_cast<size_t>(t.rows) * 8, v, DType::f32);
+      stats_of[same_as[v]] = KeptSums{t.stats_out, t.logits_slot, t.scale};
     }
-    if (forward != kNone && open(forward)) {
-      t.log_prob_slot = destinationSlot(forward);
-    } else {
-      forward = kNone;
-    }
+    if (forward != kNone) t.log_prob_slot = destinationSlot(forward);
     if (grad != kNone) {
       if (product != kNone) {
         grad = product;

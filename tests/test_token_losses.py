@@ -157,3 +157,129 @@ def test_losses_on_scaled_logits_beside_other_things(gpu_session, name, dtype, s
     for g, w, m in zip(got[1:], want[1:], magnitudes):
         w = w.reshape(g.shape)
         close(g, w, (2 * step + sums + (U[dtype] if "contraction" in name else 0)) * m + U[dtype] * np.abs(w))
+
+
+# ---------------------------------------------------------------------------------------------
+# log-probabilities that are each other's slopes
+# ---------------------------------------------------------------------------------------------
+def entangled(name):
+    """(body of (logits, tokens, other logits, other tokens), which inputs are differentiated)"""
+    mean = lambda b, x: x.sum(["s", "n"]).mul(b.scalar("f32", 1.0 / 16))  # noqa: E731
+    lp = lambda a, i, j: a[i].token_log_prob(a[j], "vocab")  # noqa: E731
+    return {
+        "weight": (lambda b, a: mean(b, lp(a, 0, 1).mul(lp(a, 2, 3).exp())), [0, 2]),
+        "product of losses": (lambda b, a: nn.cross_entropy(a[0], a[1], "vocab").mul(nn.cross_entropy(a[2], a[3], "vocab")), [0, 2]),
+        "product of sequences": (lambda b, a: lp(a, 0, 1).sum("n").mul(lp(a, 2, 3).sum("n")).sum("s").mul(b.scalar("f32", 1.0 / 256)), [0, 2]),
+        "preference": (lambda b, a: lp(a, 0, 1).sum("n").sub(lp(a, 2, 3).sum("n")).mul(b.scalar("f32", 1.0 / 32)).tanh().sum("s"), [0, 2]),
+        "two token sets": (lambda b, a: mean(b, lp(a, 0, 1).mul(lp(a, 0, 3).exp())), [0]),
+        "both weigh": (lambda b, a: mean(b, lp(a, 0, 1).mul(lp(a, 2, 3)).tanh().mul(lp(a, 2, 3).exp())), [0, 2]),
+        "three": (lambda b, a: mean(b, lp(a, 0, 1).mul(lp(a, 2, 3).exp()).mul(lp(a, 0, 3))), [0, 2]),
+        "weight and a temperature": (lambda b, a: mean(b, scaled(b, a[0], 0.5).token_log_prob(a[1], "vocab").mul(scaled(b, a[2], 2.0).token_log_prob(a[3], "vocab").exp())), [0, 2]),
+    }[name]
+
+
+ENTANGLED = ["weight", "product of losses", "product of sequences", "preference", "two token sets", "both weigh", "three", "weight and a temperature"]
+
+
+def entangled_program(name, dtype, s=2, n=3, vocab=40):
+    body, wrt = entangled(name)
+    logits, tok = T.spec(dtype, s=s, n=n, vocab=vocab), T.spec("i32", s=s, n=n)
+    return T.define("entangled", [logits, tok, logits, tok], body), wrt
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("name", ENTANGLED)
+def test_log_probabilities_in_each_others_slopes_plan(cpu_session, name, dtype):
+    program, wrt = entangled_program(name, dtype)
+    for derived in (program.value_and_grad(wrt), program.grad(wrt), program.value_and_grad(wrt[:1])):
+        calls = token_calls(plan_lines(cpu_session, derived))
+        # every value and every gradient in one kernel each at the most
+        assert 2 <= len(calls) <= 6, calls
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [(2, 3, 40), (7, 45, 5003), (3, 101, 33001)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("name", ENTANGLED)
+def test_log_probabilities_in_each_others_slopes(gpu_session, name, dtype, sizes):
+    """A log-probability of size L is off by step + L / 2^24; a product or an exponential of two of them by the sum of what they are
+    off by, relative to their sizes; what follows are sums of s * n terms.  All of it relative to the largest value of its kind."""
+    s, n, vocab = sizes
+    rng = np.random.default_rng(vocab)
+    program, wrt = entangled_program(name, dtype, s, n, vocab)
+    xs = [stored(dtype, 2.0 * rng.standard_normal((s, n, vocab))) for _ in range(2)]
+    toks = [rng.integers(-1, vocab + 1, (s, n)).astype(np.int32) for _ in range(2)]
+    inputs = [xs[0], toks[0], xs[1], toks[1]]
+    derived = program.value_and_grad(wrt)
+    got, want = run(gpu_session, derived, inputs), oracle.run(derived.wire, inputs, mode="f64")
+    top = 2.0 * max(np.abs(exactly(dtype, x)).max() for x in xs)
+    step = 2 * max(p_error(2.0 * exactly(dtype, x)) for x in xs) + 16 * U["f32"] * (top + np.log(vocab) + 1) + (s * n + 64) * U["f32"]
+    # tanh(p q) with p q above 9 is 1 to f32: its slope 1 - t * t, exactly 4 e^(-2 p q) or less, comes out of two roundings at the size
+    # of one (t within two more) and is off by up to 4 * 2^-24 whatever is left of it.  It multiplies p e^q / 16 or
+    # q e^q / 16, with e^q <= 1 and |p|, |q| <= 2 top + log(vocab).
+    saturated = 4 * U["f32"] * (2 * top + np.log(vocab)) / 16 if name == "both weigh" else 0.0
+    for g, w in zip(got, want):
+        w = w.reshape(g.shape)
+        # the log-probabilities themselves enter the slopes: errors of size step * L relative to products of size L
+        close(g, w, 4 * step * (np.abs(w) + np.abs(w).max()) * (1 + np.log(vocab)) + saturated + (U[dtype] if g.ndim else 0) * np.abs(w))
+
+
+def random_loss(seed):
+    """One to four terms of size one at most on log-probabilities of one or two logits tensors, plain or scaled, under one or two sets of
+    tokens: means, saturated ones, products of two, whole sequences, squares of the logits."""
+    rng = np.random.default_rng(7000 + seed)
+    pick = lambda *xs: xs[rng.integers(len(xs))]  # noqa: E731
+    s, n, vocab = pick(1, 2, 5), pick(1, 3, 17, 64), pick(2, 33, 130, 1003, 9001)
+    tensors, sets = pick(1, 2), pick(1, 2)
+    views = [(i, pick(None, 0.5, 3.0, -1.0, "cap")) for i in rng.integers(0, tensors, 3)]
+    terms = [(pick("mean", "tanh", "product", "weight", "sequence", "squares"), views[rng.integers(3)], int(rng.integers(sets)), views[rng.integers(3)], int(rng.integers(sets)))
+             for _ in range(rng.integers(1, 5))]
+
+    def body(b, a):
+        logits, toks = a[:tensors], a[tensors:]
+        number = lambda x: b.scalar("f32", x)  # noqa: E731
+
+        def lp(view, tok):
+            x = logits[view[0]]
+            y = x if view[1] is None else soft_capped(b, x) if view[1] == "cap" else scaled(b, x, view[1])
+            return y.token_log_prob(toks[tok], "vocab")
+        total = number(0.0)
+        for kind, v1, t1, v2, t2 in terms:
+            if kind == "squares":
+                x = logits[v1[0]]
+                term = x.mul(x).sum(["s", "n", "vocab"]).mul(number(1.0 / (16 * s * n * vocab)))
+            elif kind == "sequence":
+                term = lp(v1, t1).sum("n").mul(number(1.0 / (32 * n))).tanh().sum("s").mul(number(1.0 / s))
+            else:
+                x = lp(v1, t1)
+                x = {"mean": lambda: x.mul(number(1.0 / 32)), "tanh": lambda: x.mul(number(0.25)).tanh(), "product": lambda: x.mul(lp(v2, t2)).mul(number(1.0 / 1024)),
+                     "weight": lambda: x.mul(lp(v2, t2).exp()).mul(number(1.0 / 32))}[kind]()
+                term = x.sum(["s", "n"]).mul(number(1.0 / (s * n)))
+            total = total.add(term)
+        return total
+    specs = [T.spec("f32", s=s, n=n, vocab=vocab)] * tensors + [T.spec("i32", s=s, n=n)] * sets
+    inputs = [2.0 * rng.standard_normal((s, n, vocab)).astype(np.float32) for _ in range(tensors)] + [rng.integers(-1, vocab + 1, (s, n)).astype(np.int32) for _ in range(sets)]
+    return T.define("random", specs, body), inputs, list(range(tensors)), (s, n, vocab)
+
+
+@pytest.mark.parametrize("seed", range(64))
+def test_random_losses_plan(cpu_session, seed):
+    program, _, wrt, _ = random_loss(seed)
+    for derived in (program.value_and_grad(wrt), program.grad(wrt[:1])):
+        cpu_session.release(cpu_session.compile(derived))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(64))
+def test_random_losses_match_the_oracle(gpu_session, seed):
+    """At most four terms; each is at most one and has a slope of at most 1 / (s n) per log-probability, times a factor of at most 3 on the
+    way to the logits, and log-probabilities of size up to 32 enter the slopes divided by at least that."""
+    program, inputs, wrt, (s, n, vocab) = random_loss(seed)
+    derived = program.value_and_grad(wrt)
+    got, want = run(gpu_session, derived, inputs), oracle.run(derived.wire, inputs, mode="f64")
+    logits = [3.0 * inputs[i].astype(np.float64) for i in wrt]
+    step = 2 * max(p_error(x) for x in logits) + 16 * U["f32"] * (max(np.abs(x).max() for x in logits) + np.log(vocab) + 1) + (s * n + vocab + 64) * U["f32"]
+    close(got[0].reshape(()), float(want[0].reshape(-1)[0]), 4 * step * 4)
+    for g, w in zip(got[1:], want[1:]):
+        w = w.reshape(g.shape)
+        close(g, w, 4 * step * 4 * 3 / (s * n) + U["f32"] * np.abs(w))
