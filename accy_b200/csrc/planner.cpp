@@ -1166,13 +1166,18 @@ class Planner {
   // broadcasts, transposes and relabelling reshapes) a buffer, stopping at `except`.  What is left
   // between those buffers and `v` can then be evaluated inside another kernel.
   void materializeFolds(uint32_t v, uint32_t except = kNone) {
-    const Operation& op = P.ops[v];
-    if (sameValue(v, except) || slot_of[v] >= 0 || op.kind == Kind::constant || op.kind == Kind::iota) return;
-    if (isElementwise(op.kind) || op.kind == Kind::broadcast_in_dim || op.kind == Kind::transpose || op.kind == Kind::reshape) {
-      for (uint32_t a : op.operands) materializeFolds(a, except);
-      return;
+    std::set<uint32_t> seen;   // values share operands: each is looked at once
+    std::vector<uint32_t> stack = {v};
+    while (!stack.empty()) {
+      const uint32_t x = stack.back();
+      stack.pop_back();
+      const Operation& op = P.ops[x];
+      if (!seen.insert(x).second || sameValue(x, except) || slot_of[x] >= 0 || op.kind == Kind::constant || op.kind == Kind::iota) continue;
+      if (isElementwise(op.kind) || op.kind == Kind::broadcast_in_dim || op.kind == Kind::transpose || op.kind == Kind::reshape)
+        stack.insert(stack.end(), op.operands.rbegin(), op.operands.rend());
+      else
+        materialize(x);
     }
-    materialize(v);
   }
 
   // ---------------------------------------------------------------------------------------
@@ -1233,26 +1238,21 @@ class Planner {
   // one value under one or two names (kNone is no value's)
   bool sameValue(uint32_t a, uint32_t b) const { return a == b || (a != kNone && b != kNone && same_as[a] == same_as[b]); }
 
-  bool dependsOn(uint32_t v, uint32_t on, std::set<uint32_t>& seen) {
-    if (sameValue(v, on)) return true;
-    if (!seen.insert(v).second) return false;
-    for (uint32_t a : P.ops[v].operands)
-      if (dependsOn(a, on, seen)) return true;
-    return false;
-  }
-  bool dependsOn(uint32_t v, uint32_t on) {
-    std::set<uint32_t> seen;
-    return dependsOn(v, on, seen);
-  }
-
   // whether `v` is computed from `from` by elementwise operations and views alone
   bool elementwiseFrom(uint32_t v, uint32_t from) {
-    if (sameValue(v, from) || !dependsOn(v, from)) return true;
-    const Operation& op = P.ops[v];
-    if (!isElementwise(op.kind) && op.kind != Kind::broadcast_in_dim && op.kind != Kind::transpose && op.kind != Kind::reshape) return false;
-    for (uint32_t a : op.operands)
-      if (!elementwiseFrom(a, from)) return false;
-    return true;
+    // operations come after their operands, so one pass in order sees each once
+    std::vector<bool> depends(v + 1, false), other(v + 1, false);   // on `from`; through another kind of operation
+    for (uint32_t x = 0; x <= v; ++x) {
+      const Operation& op = P.ops[x];
+      depends[x] = sameValue(x, from);
+      if (depends[x]) continue;
+      const bool through = isElementwise(op.kind) || op.kind == Kind::broadcast_in_dim || op.kind == Kind::transpose || op.kind == Kind::reshape;
+      for (uint32_t a : op.operands) {
+        depends[x] = depends[x] || depends[a];
+        other[x] = other[x] || other[a] || (depends[a] && !through);
+      }
+    }
+    return !other[v];
   }
 
   // The slope of a gradient as an expression over its rows, with `log_prob` (if any) standing for the

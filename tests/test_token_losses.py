@@ -283,3 +283,26 @@ def test_random_losses_match_the_oracle(gpu_session, seed):
     for g, w in zip(got[1:], want[1:]):
         w = w.reshape(g.shape)
         close(g, w, 4 * step * 4 * 3 / (s * n) + U["f32"] * np.abs(w))
+
+
+# ---------------------------------------------------------------------------------------------
+# planning takes as long as a program is, not as it would be written out without shared values
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.timeout(120)
+@pytest.mark.parametrize("depth", [14, 40])
+def test_deep_shared_expressions_plan_in_time(cpu_session, depth):
+    """y -> y * tanh(y) read back without sharing has 2^depth leaves."""
+    def updates(b, a):
+        y = a[1]
+        for _ in range(depth):
+            y = y.mul(y)
+        return b.scalar("f32", 0.0).broadcast(v=5, d=8).scatter_add(a[0], y, "v")
+
+    def loss(b, a):
+        y = a[0].token_log_prob(a[1], "vocab")
+        for _ in range(depth):
+            y = y.mul(y.tanh())
+        return y.sum("n")
+    for program in (T.define("updates", [T.spec("i32", n=6), T.spec("f32", n=6, d=8)], updates),
+                    T.define("loss", [T.spec("f32", n=6, vocab=40), T.spec("i32", n=6)], loss).value_and_grad([0])):
+        cpu_session.release(cpu_session.compile(program))
