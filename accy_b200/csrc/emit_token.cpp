@@ -991,14 +991,19 @@ __device__ __forceinline__ unsigned int shared_at(const void* p) { return (unsig
 __device__ __forceinline__ void arrive(unsigned long long* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(shared_at(bar)) : "memory");
 }
-// false when the wait gave up, here or elsewhere in the CTA
+__device__ __forceinline__ bool passed(unsigned int bar, unsigned int parity) {
+  unsigned int done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0u;
+}
+#define MOST_TRIES (1u << 22)
+// false when the wait gave up, here or elsewhere in the CTA; every warp looks at `gave_up` once more before it
+// leaves, after its own last wait, and raises the status word
 __device__ __forceinline__ bool wait_for(unsigned long long* bar, unsigned int parity, volatile int* gave_up) {
   const unsigned int a = shared_at(bar);
-  for (unsigned int i = 0; i < (1u << 22); ++i) {
-    unsigned int done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done) : "r"(a), "r"(parity) : "memory");
-    if (done) return true;
+  for (unsigned int i = 0; i < MOST_TRIES; ++i) {
+    if (passed(a, parity)) return true;
     if (*gave_up) return false;
   }
   *gave_up = 1;
@@ -1106,19 +1111,14 @@ KERNEL(const XT* __restrict__ X, const TT* __restrict__ T, float* __restrict__ l
           ++issued;
         }
       }
-      if (*gave_up) {   // no copy may be in flight when the CTA leaves
-        const long long last = issued < SLOTS ? issued : SLOTS;
-        for (long long q = issued - last; q < issued; ++q) {
-          const unsigned int a = shared_at(&full[q % SLOTS]), parity = (unsigned int)((q / SLOTS) & 1);
-          for (unsigned int i = 0; i < (1u << 22); ++i) {
-            unsigned int done;
-            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                         : "=r"(done) : "r"(a), "r"(parity) : "memory");
-            if (done) break;
-          }
-        }
-        atomicExch(status, 1);
+      // no copy may be in flight when the CTA leaves, whether the consumers still wait for it or have given up
+      for (long long q = issued < SLOTS ? 0 : issued - SLOTS; q < issued; ++q) {
+        const unsigned int a = shared_at(&full[q % SLOTS]), parity = (unsigned int)((q / SLOTS) & 1);
+        unsigned int i = 0;
+        while (i < MOST_TRIES && !passed(a, parity)) ++i;
+        if (i == MOST_TRIES) *gave_up = 1;
       }
+      if (*gave_up) atomicExch(status, 1);
     }
     return;
   }
@@ -1224,6 +1224,7 @@ KERNEL(const XT* __restrict__ X, const TT* __restrict__ T, float* __restrict__ l
     }
 #endif
   }
+  if (lane == 0 && *gave_up) atomicExch(status, 1);
 }
 )CUDA";
 

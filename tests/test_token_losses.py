@@ -306,3 +306,26 @@ def test_deep_shared_expressions_plan_in_time(cpu_session, depth):
     for program in (T.define("updates", [T.spec("i32", n=6), T.spec("f32", n=6, d=8)], updates),
                     T.define("loss", [T.spec("f32", n=6, vocab=40), T.spec("i32", n=6)], loss).value_and_grad([0])):
         cpu_session.release(cpu_session.compile(program))
+
+
+# ---------------------------------------------------------------------------------------------
+# the streaming kernel
+# ---------------------------------------------------------------------------------------------
+def streaming_source(session):
+    specs = [T.spec("bf16", n=4096, vocab=131072), T.spec("i32", n=4096)]
+    compiled = session.compile(T.define("ce", specs, lambda b, a: nn.cross_entropy(a[0], a[1], "vocab")).value_and_grad([0]))
+    sources = [text for _, text, _ in compiled.kernels() if "cp.async.bulk" in text]
+    session.release(compiled)
+    assert len(sources) == 1
+    return sources[0]
+
+
+def test_every_warp_of_the_streaming_kernel_reports_a_wait_that_gave_up(cpu_session):
+    """Every warp raises the session's status word after its own last wait, the producer's and each consumer's: the others may
+    have ended before a wait runs out.  (No test makes one run out on a device: that would take a kernel that hangs.)"""
+    source = streaming_source(cpu_session)
+    producer, consumers = source[source.index("KERNEL(const XT*"):].split("  // Consumers.")
+    for part in (producer, consumers):
+        last_wait = max(part.rindex("wait_for(&"), part.rindex("passed(") if "passed(" in part else 0)
+        assert "*gave_up) atomicExch(status, 1);" in part[last_wait:]
+    assert source.count("atomicExch(status, 1)") == 2
