@@ -624,8 +624,15 @@ namespace {
 // or divided by the sum, so its rounding cancels, and the fused step rounds at the size of its result: rows whose
 // logits are all far from zero lose nothing.  References are combined as 2^(c1 - c2), for the same
 // reason.  A reference of 1e34 or more might overflow c: such rows (logits at the type's lowest value)
-// subtract first.  Where the logits are others times a number, the number goes into the constant (L2E below).  A thread moves its reference only when a logit exceeds it by more than 40: e^40 times
-// any number of terms is far from the end of f32, and the sums then rarely need rescaling.
+// subtract first.  Where the logits are others times a number, the number goes into the constant (L2E below).
+//
+// An exponent is rounded at its own size, so a reference that lies d below the row's maximum costs the largest terms d times
+// 2^-24 or so.  A thread moves its reference when a logit exceeds it by more than 4, which happens a few times per row, and
+// adds what comes after a new reference to a sum of its own: the many small terms beside a token
+// the model is sure of are not rounded one by one at the size of that token's.  Log-probabilities of such rows are within 5e-7
+// (largest of 600 rows each of 32003 to 300007 logits; with a window of 40 and one sum 4e-6, some of them
+// positive).  bf16 8192 x 131072 with the gradient: 721 us, 707 with the window of 40.  An exact running maximum gained no
+// more (730 us), nor did compensated sums (732 us).
 const char* kTokenCommon = R"CUDA(
 #define LN2 0.6931471805599453f
 #define NEG_INF __uint_as_float(0xff800000u)
@@ -704,10 +711,10 @@ template <bool HUGE> __device__ __forceinline__ void exps(const Raw& v, float m,
     f[e + 1] = ex2_ftz(b);
   }
 }
-// a thread's share of a row's sum
+// a thread's share of a row's sum: s + rest relative to m.  `rest` is what was added since m last moved.
 struct Sum {
-  float m, s, limit;
-  __device__ __forceinline__ Sum() : m(NEG_INF), s(0.0f), limit(NEG_INF) {}
+  float m, s, limit, rest, minus;
+  __device__ __forceinline__ Sum() : m(NEG_INF), s(0.0f), limit(NEG_INF), rest(0.0f), minus(0.0f) {}
   template <int N> __device__ __forceinline__ void fold(const Raw (&raw)[N]) {
     unsigned int top = raw[0].w[0];
 #pragma unroll
@@ -715,27 +722,33 @@ struct Sum {
 #pragma unroll
       for (int q = 0; q < 4; ++q) top = packed_max(top, raw[i].w[q]);
     const float t = largest(top);
-    if (t > limit) {
-      s = moved(s, m, t);
+    const bool top_here = t > limit;
+    if (top_here) {
+      s = moved(s + rest, m, t);
+      rest = 0.0f;
       m = t;
-      limit = t + 40.0f / SCALE;
+      minus = minus_c(t);
+      limit = t + 4.0f / SCALE;
     }
-    if (huge_ref(m)) add<true>(raw);
-    else add<false>(raw);
+    if (huge_ref(m)) add<true>(raw, top_here);
+    else add<false>(raw, top_here);
   }
-  template <bool HUGE, int N> __device__ __forceinline__ void add(const Raw (&raw)[N]) {
-    const float minus = minus_c(m);
-    unsigned long long acc = pk2(s, 0.0f);
+  template <bool HUGE, int N> __device__ __forceinline__ void add(const Raw (&raw)[N], bool top_here) {
+    unsigned long long acc;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float f[E];
       exps<HUGE>(raw[i], m, minus, f);
 #pragma unroll
-      for (int e = 0; e < E; e += 2) acc = add2(acc, pk2(f[e], f[e + 1]));
+      for (int e = 0; e < E; e += 2) {
+        const unsigned long long pair = pk2(f[e], f[e + 1]);
+        acc = i + e == 0 ? pair : add2(acc, pair);
+      }
     }
     float lo, hi;
     upk2(acc, lo, hi);
-    s = lo + hi;
+    if (top_here) s = s + (lo + hi);
+    else rest = rest + (lo + hi);
   }
   // the sum over W neighbouring lanes, in every one of them
   template <int W> __device__ __forceinline__ void across_lanes() {
@@ -746,7 +759,8 @@ struct Sum {
 #pragma unroll
       for (int off = W / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off, W));
     }
-    s = moved(s, m, top);
+    s = moved(s + rest, m, top);
+    rest = 0.0f;
     m = top;
 #pragma unroll
     for (int off = W / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off, W);
@@ -756,7 +770,8 @@ struct Sum {
 // difference is taken before anything is rounded at the size of x.
 __device__ __forceinline__ float log_prob_at(float x, float m, float total) {
   const float residue = huge_ref(m) ? 0.0f : __fmaf_rn(m, L2E, minus_c(m));
-  return (x - m) * SCALE - (logf(total) - residue * LN2);
+  const float log_prob = (x - m) * SCALE - (logf(total) - residue * LN2);
+  return log_prob > 0.0f ? 0.0f : log_prob;   // a probability of one, rounded
 }
 
 #if GRADIENT

@@ -8,7 +8,7 @@ import pytest
 
 from accy_b200 import nn, tensor
 from oracle import oracle
-from test_token_programs import close, exactly, p_error, plan_lines, run, stored, U
+from test_token_programs import TINY, U, close, exactly, log_prob_of, p_error, plan_lines, run, stored
 
 T = tensor
 
@@ -329,3 +329,61 @@ def test_every_warp_of_the_streaming_kernel_reports_a_wait_that_gave_up(cpu_sess
         last_wait = max(part.rindex("wait_for(&"), part.rindex("passed(") if "passed(" in part else 0)
         assert "*gave_up) atomicExch(status, 1);" in part[last_wait:]
     assert source.count("atomicExch(status, 1)") == 2
+
+
+# ---------------------------------------------------------------------------------------------
+# rows where the model is sure of its token
+# ---------------------------------------------------------------------------------------------
+def sure_rows(dtype, n, vocab, gap, seed):
+    """Logits of deviation 2.5 with one token `gap` above their mean, at the ends of the row and in between"""
+    rng = np.random.default_rng(seed)
+    x = 2.5 * rng.standard_normal((n, vocab))
+    tok = rng.integers(0, vocab, (n,)).astype(np.int32)
+    tok[:4] = [0, 1, vocab // 2, vocab - 1]
+    x[np.arange(n), tok] = gap
+    return stored(dtype, x), tok
+
+
+def sure_error(gap, p):
+    """What log p of such a token may be off by.  Its own term: the exponent is rounded at a distance of at most 4 from the
+    reference (half a step of [4, 8) is 2^-22, in units of log2), log2(e) is off by 1.4e-8 relative, ex2 by 2^-22.  The sum:
+    fifteen additions at the size of the total, and terms up to 45 below it, off by 45 * log2(e) * 2^-24 + 2^-22 each, which are
+    1 - p of it.  The logarithm: half a step of [2, 4) and the rounding of the difference.  Where the other terms
+    add up to less than half a step of one, nothing is added to a token's term of exactly one: ex2 near zero and two roundings."""
+    if gap >= 40:
+        return 2.0 ** -22 + 2 * U["f32"]
+    own = 2.0 ** -22 * np.log(2) + 4 * 1.4e-8 + 2.0 ** -22
+    return own + 15 * U["f32"] + (1 - p) * (45 * 1.4427 * U["f32"] + 2.0 ** -22) + 2.0 ** -23 + U["f32"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [18.0, 25.0, 32.0, 40.0])
+@pytest.mark.parametrize("dtype,n,vocab", [("bf16", 40, 131072), ("f32", 40, 300007), ("f16", 700, 50001), ("bf16", 300, 131072), ("f32", 310, 32003), ("bf16", 60, 5003)])
+def test_log_probabilities_near_zero(gpu_session, dtype, n, vocab, gap):
+    """Few rows are held in registers, split over a cluster or read in chunks; more than two per SM pass through shared memory where a
+    gradient is asked for; a slope over all rows takes the kept sums."""
+    x, tok = sure_rows(dtype, n, vocab, gap, int(gap) + n)
+    want, p, hot, _ = log_prob_of(exactly(dtype, x), tok)
+    at = np.arange(n), tok
+    p_tok = p[at]
+    allowed = sure_error(gap, p_tok)
+    specs = [T.spec(dtype, n=n, vocab=vocab), T.spec("i32", n=n)]
+
+    def value(b, a):
+        return a[0].token_log_prob(a[1], "vocab")
+
+    def total(b, a):
+        return value(b, a).sum("n")
+
+    def sequence(b, a):
+        return value(b, a).sum("n").mul(b.scalar("f32", 2.0 ** -20)).tanh()
+    got = run(gpu_session, T.define("value", specs, value), [x, tok])[0]
+    assert np.all(got <= 0)
+    close(got, want, allowed)
+    # at the token the gradient is 1 - p, which is what log p has lost
+    for body, slope in ((total, 1.0), (sequence, 2.0 ** -20)):
+        grad = run(gpu_session, T.define("loss", specs, body).grad([0]), [x, tok])[0]
+        exact = slope * (1 - p_tok)
+        # the slope of the whole sequence is 2^-20 * (1 - tanh(2^-20 * sum)^2): within 2^-24 of 2^-20 for a sum below 2^8
+        assert np.abs(want).sum() < 2.0 ** 8
+        close(grad[at], exact, slope * allowed + (U[dtype] + 2.0 ** -20 + 4 * U["f32"]) * exact + TINY[dtype])
