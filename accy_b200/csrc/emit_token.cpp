@@ -1246,7 +1246,9 @@ KERNEL(const XT* __restrict__ X, const TT* __restrict__ T, float* __restrict__ l
 }  // namespace
 
 void emitTokenLogProb(const TokenOp& op, const std::string& name, Plan& plan, const ScheduleOverrides& ov) {
-  if (op.vocab > 0x7ff00000ll) throw PlanError("token log-probabilities over more than 2^31 - 2^20 entries are not supported");
+  // Elements of a row are counted in 32 bits, up to the end of the last chunk of the last part: 64 parts of whole chunks of
+  // 4096 vectors of 8 elements reach less than 2^21 elements past the row.
+  if (op.vocab > 0x7fc00000ll) throw PlanError("token log-probabilities over more than 2^31 - 2^22 entries are not supported");
   const int in_size = static_cast<int>(dtypeSize(op.logits_dtype)), e = 16 / in_size;
   // aligned vectors that cover a row, wherever it starts
   const int64_t vectors = op.vocab % e == 0 ? op.vocab / e : (op.vocab + 2 * e - 2) / e;

@@ -387,3 +387,32 @@ def test_log_probabilities_near_zero(gpu_session, dtype, n, vocab, gap):
         # the slope of the whole sequence is 2^-20 * (1 - tanh(2^-20 * sum)^2): within 2^-24 of 2^-20 for a sum below 2^8
         assert np.abs(want).sum() < 2.0 ** 8
         close(grad[at], exact, slope * allowed + (U[dtype] + 2.0 ** -20 + 4 * U["f32"]) * exact + TINY[dtype])
+
+
+# ---------------------------------------------------------------------------------------------
+# the largest vocabularies
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [1, 300])
+def test_elements_of_the_longest_rows_are_counted_in_32_bits(cpu_session, dtype, n):
+    def kernels(vocab, body):
+        specs = [T.spec(dtype, n=n, vocab=vocab), T.spec("i32", n=n)]
+        compiled = cpu_session.compile(T.define("long", specs, body).grad([0]))
+        sources = [text for _, text, _ in compiled.kernels() if "#define VOCAB" in text]
+        cpu_session.release(compiled)
+        return sources
+    bodies = [lambda b, a: a[0].token_log_prob(a[1], "vocab").sum("n"), lambda b, a: a[0].token_log_prob(a[1], "vocab").sum("n").tanh()]
+    for body in bodies:
+        for source in kernels(2 ** 31 - 2 ** 22, body):
+            number = lambda name: int(source.split("#define %s " % name)[1].split("\n")[0])  # noqa: E731,B023
+            e, vocab = number("E"), number("VOCAB")
+            vectors = vocab // e             # rows of whole vectors
+            if "#define CHUNK " in source:   # whole chunks of one row
+                reach = -(-vectors // number("CHUNK")) * number("CHUNK")
+            else:                            # whole chunks of every part
+                reach = number("PARTS") * number("CHUNKS") * number("TPR") * number("VPT")
+            assert vectors <= reach and (reach + 1) * e < 2 ** 31
+        for vocab in (2 ** 31 - 2 ** 21, 2 ** 31 - 2 ** 20):
+            with pytest.raises(T.SessionError) as err:
+                kernels(vocab, body)
+            assert err.value.name == "compile_failed" and "not supported" in err.value.message
