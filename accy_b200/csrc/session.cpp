@@ -6,6 +6,7 @@
 // what the reference's LoadedFragment owns (src/executable/fragment.zig:711-757): the loaded
 // kernels, the planned device slots and the launch list.  There is no CPU fallback anywhere:
 // without a CUDA device the session can only compile.
+#include <algorithm>
 #include <chrono>
 #include <cstdlib>
 #include <cstring>
@@ -48,11 +49,15 @@ struct Entry {
   std::vector<std::vector<std::string>> names;  // descriptor name storage
   CUevent_t ev_begin = nullptr, ev_end = nullptr;
   bool timed = false;
-  // The launch list recorded once as a CUDA graph and replayed while the bound pointers stay the
-  // same (a host invoke always binds the program's own buffers).
+  // The launch list recorded as a CUDA graph and replayed while the bound pointers stay the same (a host
+  // invoke always binds the program's own buffers).  Recording costs as much as ten or twenty plain
+  // launches of the list, so it waits until the same pointers have come again, twice as often for every further recording:
+  // a caller that changes buffers every time is never recorded, one whose buffers settle always is.
   CUgraphExec_t graph = nullptr;
-  std::vector<CUdeviceptr_t> graph_bound;
-  int graph_recordings = 0;              // re-recordings so far; callers that change pointers every time stop being recorded
+  std::vector<CUdeviceptr_t> graph_bound, last_bound;
+  int last_bound_calls = 0;              // calls in a row with last_bound, none of them replayed
+  int graph_recordings = 0;
+  bool graphs_refused = false;           // the driver failed to record or to replay: plain launches from then on
   // Encoded tensor maps, one per (launch, argument), kept while the pointer they were encoded for
   // stays bound: a steady invoke loop does no cuTensorMapEncodeTiled on its launch path.
   struct CachedMap {
@@ -388,10 +393,10 @@ struct accy_b200_session {
   }
 
   // Launches the plan with e.bound holding a device pointer for every slot.  A plan of several
-  // kernels is recorded as a CUDA graph on its first single-shot launch and replayed afterwards
-  // (one submission instead of one per kernel; the reference's record_sequence / submit_sequence,
+  // kernels is recorded as a CUDA graph, on its first single-shot launch from the program's own buffers or when
+  // a caller's buffers come again, and replayed afterwards (one submission instead of one per kernel; the reference's record_sequence / submit_sequence,
   // deps/lib/compiler/gpu/src/contract.zig:1929-1966).  ACCY_B200_NO_GRAPHS=1 turns this off.
-  void launchAll(Entry& e, CUstream_t on, bool time_it) {
+  void launchAll(Entry& e, CUstream_t on, bool time_it, bool own_buffers = true) {
     if (poisoned) throw StatusError{ACCY_B200_LAUNCH_FAILED, "session is poisoned by an earlier failed launch"};
     const DriverTable& d = driver();
     // Events around the launch list cost the stream a few microseconds per invoke (each one
@@ -399,16 +404,27 @@ struct accy_b200_session {
     const bool record_events = time_it && time_launches;
     if (record_events) check(d.cuEventRecord(e.ev_begin, on), "cuEventRecord");
     static const bool graphs_off = std::getenv("ACCY_B200_NO_GRAPHS") != nullptr;
-    bool replayable = time_it && !graphs_off && e.plan.launches.size() >= 2 && e.graph_recordings < 4;
+    bool replayable = time_it && !graphs_off && e.plan.launches.size() >= 2 && !e.graphs_refused;
     // A stream that the caller is capturing takes the kernels themselves: its own graph replays them, and
     // neither a recording nor a graph launch may happen in the middle of it.
     int capturing = 0;
     if (replayable && d.cuStreamIsCapturing(on, &capturing) == 0 && capturing != 0) replayable = false;
-    bool submitted = false;
-    if (replayable && e.graph && e.graph_bound == e.bound) {
+    bool submitted = false, record = false;
+    const bool recorded_before = replayable && e.graph && e.graph_bound == e.bound;
+    if (recorded_before) {
+      e.last_bound_calls = 0;
+    } else if (replayable) {
+      if (e.last_bound != e.bound) {
+        e.last_bound = e.bound;
+        e.last_bound_calls = 0;
+      }
+      e.last_bound_calls += 1;
+      record = e.last_bound_calls >= (2 << std::min(e.graph_recordings, 16)) || (own_buffers && e.graph_recordings == 0);
+    }
+    if (recorded_before) {
       submitted = d.cuGraphLaunch(e.graph, on) == 0;
-      if (!submitted) e.graph_recordings = 4;  // give up on graphs for this program, launch directly below
-    } else if (replayable && d.cuStreamBeginCapture(stream, 2 /* relaxed: other threads' calls do not matter */) == 0) {
+      e.graphs_refused = !submitted;   // launched directly below
+    } else if (record && d.cuStreamBeginCapture(stream, 2 /* relaxed: other threads' calls do not matter */) == 0) {
       // recorded on the session's own stream: the legacy default stream (handle 1) cannot be captured
       if (e.graph) d.cuGraphExecDestroy(e.graph);
       e.graph = nullptr;
@@ -428,7 +444,7 @@ struct accy_b200_session {
       } else {
         if (e.graph) d.cuGraphExecDestroy(e.graph);
         e.graph = nullptr;
-        e.graph_recordings = 4;
+        e.graphs_refused = true;
       }
       if (recorded) d.cuGraphDestroy(recorded);
     }
@@ -720,7 +736,7 @@ uint32_t accy_b200_session_invoke_device(accy_b200_session* s, uint64_t handle, 
       if (output_ptrs[j] % ACCY_B200_BUFFER_ALIGNMENT) throw StatusError{ACCY_B200_INVALID_BUFFER, "output pointer is not 256-byte aligned"};
       e.bound[e.plan.output_slots[j]] = output_ptrs[j];
     }
-    s->launchAll(e, stream ? static_cast<CUstream_t>(stream) : s->stream, true);
+    s->launchAll(e, stream ? static_cast<CUstream_t>(stream) : s->stream, true, /*own_buffers=*/false);
   });
 }
 
