@@ -627,12 +627,13 @@ namespace {
 // subtract first.  Where the logits are others times a number, the number goes into the constant (L2E below).
 //
 // An exponent is rounded at its own size, so a reference that lies d below the row's maximum costs the largest terms d times
-// 2^-24 or so.  A thread moves its reference when a logit exceeds it by more than 4, which happens a few times per row, and
-// adds what comes after a new reference to a sum of its own: the many small terms beside a token
-// the model is sure of are not rounded one by one at the size of that token's.  Log-probabilities of such rows are within 5e-7
-// (largest of 600 rows each of 32003 to 300007 logits; with a window of 40 and one sum 4e-6, some of them
-// positive).  bf16 8192 x 131072 with the gradient: 721 us, 707 with the window of 40.  An exact running maximum gained no
-// more (730 us), nor did compensated sums (732 us).
+// 2^-24 or so.  A thread moves its reference when a logit exceeds it by more than 5.5 (exponents of the largest
+// terms then stay below 8), and adds what comes after a new reference to a sum of its own: the many small terms beside
+// a token the model is sure of are not rounded one by one at the size of that token's.  Log-probabilities of such
+// rows are within 6e-7 (the largest of 600 rows each of 32003 to 300007 logits, the token 14 to 40 above the mean; with
+// a window of 40 and one sum 4e-6, some of them positive).  bf16 8192 x 131072 with the gradient 708 us, f32
+// 1023 x 32003 56.0 us (with the window of 40 and one sum 712 and 55.4; with 4, which moves it more often, 720 and 57.3;
+// with an exact running maximum 730 and 57.4; with compensated sums 732 and 57.4, without smaller errors).
 const char* kTokenCommon = R"CUDA(
 #define LN2 0.6931471805599453f
 #define NEG_INF __uint_as_float(0xff800000u)
@@ -728,7 +729,7 @@ struct Sum {
       rest = 0.0f;
       m = t;
       minus = minus_c(t);
-      limit = t + 4.0f / SCALE;
+      limit = t + 5.5f / SCALE;
     }
     if (huge_ref(m)) add<true>(raw, top_here);
     else add<false>(raw, top_here);

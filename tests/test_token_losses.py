@@ -345,15 +345,16 @@ def sure_rows(dtype, n, vocab, gap, seed):
 
 
 def sure_error(gap, p):
-    """What log p of such a token may be off by.  Its own term: the exponent is rounded at a distance of at most 4 from the
-    reference (half a step of [4, 8) is 2^-22, in units of log2), log2(e) is off by 1.4e-8 relative, ex2 by 2^-22.  The sum:
-    fifteen additions at the size of the total, and terms up to 45 below it, off by 45 * log2(e) * 2^-24 + 2^-22 each, which are
-    1 - p of it.  The logarithm: half a step of [2, 4) and the rounding of the difference.  Where the other terms
-    add up to less than half a step of one, nothing is added to a token's term of exactly one: ex2 near zero and two roundings."""
+    """What log p of such a token may be off by.  Its own term: the token lies at most 5.5 above its reference, an exponent below 8 is
+    rounded by at most half a step of [4, 8) (2^-22, in units of log2), log2(e) is off by 1.4e-8 relative, ex2 by 2^-22.  The
+    sum: fifteen additions at the size of the total, and terms up to 45 below it, off by 45 * log2(e) * 2^-24 + 2^-22 each,
+    which are 1 - p of it.  The logarithm, at most 5.5: half a step of [4, 8) is 2^-22, and the rounding of the difference.
+    40 above: the reference is the token itself, and the other terms add up to less than half a step of one, so nothing is added
+    to a term of exactly one: ex2 near zero and two roundings."""
     if gap >= 40:
         return 2.0 ** -22 + 2 * U["f32"]
-    own = 2.0 ** -22 * np.log(2) + 4 * 1.4e-8 + 2.0 ** -22
-    return own + 15 * U["f32"] + (1 - p) * (45 * 1.4427 * U["f32"] + 2.0 ** -22) + 2.0 ** -23 + U["f32"]
+    own = 2.0 ** -22 * np.log(2) + 5.5 * 1.4e-8 + 2.0 ** -22
+    return own + 15 * U["f32"] + (1 - p) * (45 * 1.4427 * U["f32"] + 2.0 ** -22) + 2.0 ** -22 + U["f32"]
 
 
 @pytest.mark.gpu
