@@ -1122,8 +1122,8 @@ class Planner {
       s.base_slot = materialize(base);
       s.base_dtype = plan.slots[s.base_slot].storage;
     }
-    // The updates: the elementwise ops that compute them are evaluated where they are summed, unless
-    // another kernel needs them too or they are not elementwise all the way.
+    // The updates: the elementwise ops that compute them are evaluated where they are summed (and once more wherever
+    // else they are needed), unless they see their operands in a way that this kernel cannot.
     Build b;
     b.root = updates;
     std::vector<int> map(ut.rank());
