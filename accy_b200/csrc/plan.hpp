@@ -117,7 +117,7 @@ struct TokenOp {
   int logits_slot = -1, token_slot = -1;
   DType logits_dtype = DType::f32, token_dtype = DType::i32;   // storage types
   int log_prob_slot = -1;         // written when >= 0
-  int stats_out = -1, stats_in = -1;  // (row maximum, sum of exponentials) written / read in place of a pass
+  int stats_out = -1, stats_in = -1;  // (reference near the row's maximum, sum relative to it) written / read in place of a pass
   int grad_slot = -1;             // written when >= 0
   float scale = 1.0f;             // the log-probabilities are those of logits * scale (scale > 0)
   float grad_scale = 1.0f;        // the gradient is written times this

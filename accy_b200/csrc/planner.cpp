@@ -1184,7 +1184,7 @@ class Planner {
   // log-probabilities of tokens, and their gradient
   // ---------------------------------------------------------------------------------------
   static constexpr uint32_t kNone = 0xffffffffu;
-  // Rows' maxima and sums that a log-probability's kernel has left, with the logits and the factor they were made from:
+  // Rows' references and sums that a log-probability's kernel has left, with the logits and the factor they were made from:
   // a product may get a buffer of its own after one call was planned and before the next, and sums of
   // x times a factor are no sums of the product.
   struct KeptSums {
@@ -1313,7 +1313,7 @@ class Planner {
       both = may_join && elementwiseFrom(P.ops[grad].operands[2], forward) && slopeOf(P.ops[grad].operands[2], forward, &t.slope);
       if (!both && is_grad) {
         // the slope needs log-probabilities of other rows: they come first, in a kernel of their own,
-        // which leaves its rows' maxima and sums for this one
+        // which leaves its rows' references and sums for this one
         materializeFolds(any.operands[2]);
         forward = kNone;
         t.slope = Epilogue{};
